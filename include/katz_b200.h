@@ -333,6 +333,57 @@ int katz_euler_scale_input(const void* x, void* out, long long n, float sigma, i
 int katz_euler_cfg_step(void* x, const void* eps_uncond, const void* eps_cond, long long n, float guidance, float sigma,
                         float sigma_next, int mode, void* stream);
 
+/* --------------------------------------------------------------------------------------------- 4-bit weights ---- */
+/* A weight matrix [N, K], K % 32 == 0, in 4 bits: q[N, K/2] bytes (code of an even k in the low four bits), scale[N, J] in
+ * bf16 and zero[N, J] bytes (0..15; NULL = 8 everywhere) for J = ceil(K / group) groups of `group` = 32, 64 or 128
+ * consecutive k (the last may be short): w = scale * (code - zero). All three are contiguous; q is 16-byte aligned. */
+
+/* fp16 [N, K] (row stride ldw) -> q, scale: scale = bf16(max |w| / 7) of the group, code = 8 + rint(w / scale), ties to even. A
+ * group with an infinity or a NaN gets a NaN scale. w is 16-byte aligned and ldw % 8 == 0. */
+int katz_quantize_w4_f16(const void* w, long long ldw, void* q, void* scale, int N, int K, int group, void* stream);
+/* fp16(scale * (code - zero)) -> w [N, K] (row stride ldw, 16-byte aligned rows). */
+int katz_dequantize_w4_f16(const void* q, const void* scale, const void* zero, void* w, long long ldw, int N, int K, int group,
+                           void* stream);
+/* out[M, N] = (act(x W^T + bias) + residual) * out_scale with W in 4 bits, fp32 accumulation, any M and N. x, out and
+ * residual are row-strided (strides in elements, rows do not overlap); residual may be out, x may not. The weight enters the
+ * product as an fp16 value of 64 * w: exact for |scale| from 2^-23 to 64 without zero points (with them, code - zero = 9, 11, 13
+ * and 15 round in the 12th bit); larger weights than 1023 overflow to infinity. */
+int katz_linear_w4_f16(const void* x, long long ldx, const void* q, const void* scale, const void* zero, int group, void* out,
+                       long long ldo, int M, int N, int K, const void* bias, const void* residual, long long ldr, int act,
+                       float out_scale, void* stream);
+
+/* ------------------------------------------------------------------------------- norms around a gated residual ---- */
+#define KATZ_NORM_NONE 0
+#define KATZ_NORM_LAYER 1
+#define KATZ_NORM_RMS 2
+#define KATZ_RESIDUAL_NORM_MAX_C 16384
+
+/* u = post(y); h = residual_scale * x + gate * u; z = pre(h) * (1 + scale) + shift, over [B, S, C] with unit channel stride and
+ * batch / token strides (in elements; 0 broadcasts gate, scale and shift). x and h are fp16 or fp32 (x_dtype), everything else
+ * fp16. Optional (NULL): y (then h = residual_scale * x, post_kind 0 and no gate), gate, scale, shift, weights, biases, h
+ * (not stored), z (exactly when pre_kind is 0). Statistics are fp32, of the unrounded h. h may be x and z may be y (the same
+ * strides); other overlaps are not allowed. */
+typedef struct katz_residual_norm_args {
+    const void* x;
+    const void* y;
+    const void* gate;
+    const void* scale;
+    const void* shift;
+    const void* post_weight;
+    const void* post_bias;
+    const void* pre_weight;
+    const void* pre_bias;
+    void* h;
+    void* z;
+    long long x_sb, x_ss, y_sb, y_ss, h_sb, h_ss, z_sb, z_ss, gate_sb, gate_ss, scale_sb, scale_ss, shift_sb, shift_ss;
+    int B, S, C;
+    int x_dtype;
+    int post_kind, pre_kind;
+    float post_eps, pre_eps;
+    float residual_scale;
+} katz_residual_norm_args;
+int katz_residual_norm_f16(const katz_residual_norm_args* h_args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

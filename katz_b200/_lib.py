@@ -14,6 +14,10 @@ KATZ_DTYPE_F32 = 1
 ACT_NONE = 0
 ACT_SILU = 1
 LORA_MAX_ADAPTERS = 4
+NORM_NONE = 0
+NORM_LAYER = 1
+NORM_RMS = 2
+RESIDUAL_NORM_MAX_C = 16384
 
 _ERRORS = {
     -1: "invalid argument (null pointer or bad enum)",
@@ -50,6 +54,15 @@ _V, _I, _L, _F = c_void_p, c_int, c_longlong, c_float
 class LinearExtras(Structure):
     """Mirror of `struct katz_linear_extras`."""
     _fields_ = [("ln_stats", c_void_p), ("ln_c12", c_void_p), ("ln_slots", c_int), ("ln_eps", c_float), ("stats_out", c_void_p)]
+
+
+class ResidualNormArgs(Structure):
+    """Mirror of `struct katz_residual_norm_args`."""
+    _fields_ = ([(n, c_void_p) for n in ("x", "y", "gate", "scale", "shift", "post_weight", "post_bias", "pre_weight", "pre_bias", "h", "z")]
+                + [(n, c_longlong) for n in ("x_sb", "x_ss", "y_sb", "y_ss", "h_sb", "h_ss", "z_sb", "z_ss", "gate_sb", "gate_ss",
+                                             "scale_sb", "scale_ss", "shift_sb", "shift_ss")]
+                + [(n, c_int) for n in ("B", "S", "C", "x_dtype", "post_kind", "pre_kind")]
+                + [(n, c_float) for n in ("post_eps", "pre_eps", "residual_scale")])
 
 
 # name -> (restype, argtypes). Every symbol include/katz_b200.h declares must be listed here; a test checks it.
@@ -115,6 +128,10 @@ SIGNATURES = {
     "katz_nhwc_to_nchw_f16": (_I, [_V, _V, _I, _I, _I, _I, _V]),
     "katz_euler_scale_input": (_I, [_V, _V, _L, _F, _I, _I, _V]),
     "katz_euler_cfg_step": (_I, [_V, _V, _V, _L, _F, _F, _F, _I, _V]),
+    "katz_quantize_w4_f16": (_I, [_V, _L, _V, _V, _I, _I, _I, _V]),
+    "katz_dequantize_w4_f16": (_I, [_V, _V, _V, _V, _L, _I, _I, _I, _V]),
+    "katz_linear_w4_f16": (_I, [_V, _L, _V, _V, _V, _I, _V, _L, _I, _I, _I, _V, _V, _L, _I, _F, _V]),
+    "katz_residual_norm_f16": (_I, [POINTER(ResidualNormArgs), _V]),
 }
 
 _lib = None

@@ -180,6 +180,124 @@ def linear(x, w, bias=None, residual=None, act=ACT_NONE, rowvec=None, rows_per_b
     return out
 
 
+def _same_device(t, device, name):
+    if t.device != device:
+        raise KatzError("%s is on %s, not on %s" % (name, t.device, device))
+    return t
+
+
+def _call_on(device, name, *args):
+    """Launch on the current stream of `device`, which need not be the current device."""
+    if device.index == torch.cuda.current_device():
+        call(name, *args, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+        return
+    with torch.cuda.device(device):
+        call(name, *args, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+
+
+def _rows_ok(t, M, N):
+    """[M, N] with unit column stride and rows that do not overlap."""
+    return t.dim() == 2 and t.shape == (M, N) and (t.stride(1) == 1 or N == 1) and (M < 2 or t.stride(0) >= N)
+
+
+def _w4_check(what, q, scale, zero, group):
+    """(N, K) of a 4-bit weight; see quantize_w4 for the format."""
+    if group not in (32, 64, 128):
+        raise KatzError("%s: group must be 32, 64 or 128 (got %r)" % (what, group))
+    if q.dtype != torch.uint8 or not q.is_cuda or q.dim() != 2 or not q.is_contiguous():
+        raise KatzError("%s: q must be a contiguous CUDA uint8 [N, K/2] tensor" % what)
+    N, K = q.shape[0], 2 * q.shape[1]
+    if K == 0 or K % 32:
+        raise KatzError("%s: K must be a positive multiple of 32 (got %d)" % (what, K))
+    if q.data_ptr() % 16:
+        raise KatzError("%s: q must start on a 16-byte boundary" % what)
+    shape = (N, (K + group - 1) // group)
+    if scale.dtype != torch.bfloat16 or scale.shape != shape or not scale.is_contiguous():
+        raise KatzError("%s: scale must be a contiguous bf16 [N, ceil(K/group)] = %s tensor" % (what, shape))
+    _same_device(scale, q.device, "scale")
+    if zero is not None:
+        if zero.dtype != torch.uint8 or zero.shape != shape or not zero.is_contiguous():
+            raise KatzError("%s: zero must be a contiguous uint8 %s tensor" % (what, shape))
+        _same_device(zero, q.device, "zero")
+    return N, K
+
+
+def quantize_w4(w, group=64, out=None):
+    """fp16 weights [N, K] -> (q, scale), 4 bits a weight. K is a multiple of 32; w may be row-strided.
+    q: uint8 [N, K/2], two codes a byte, the even k in the low four bits; scale: bf16 [N, ceil(K/group)], one for `group` (32,
+    64 or 128) consecutive k of a row, the last group may be short; weight = scale * (code - 8), |code - 8| <= 7, ties to even.
+    A group that holds an infinity or a NaN reads back as NaN. Rows are independent: row slices of (q, scale) are the 4-bit
+    form of the same rows of w. `out` = (q, scale) rewrites an existing pair, as after an adapter switch."""
+    _f16(w, "w")
+    if w.dim() != 2 or w.shape[1] == 0 or w.shape[1] % 32:
+        raise KatzError("quantize_w4: w must be [N, K] with K a positive multiple of 32 (got %s)" % (tuple(w.shape),))
+    N, K = w.shape
+    if not _rows_ok(w, N, K) or not _al16(w) or (N > 1 and w.stride(0) % 8):
+        raise KatzError("quantize_w4: w must have unit column stride and 16-byte aligned rows")
+    if group not in (32, 64, 128):
+        raise KatzError("quantize_w4: group must be 32, 64 or 128 (got %r)" % (group,))
+    if out is None:
+        out = (torch.empty((N, K // 2), dtype=torch.uint8, device=w.device),
+               torch.empty((N, (K + group - 1) // group), dtype=torch.bfloat16, device=w.device))
+    q, scale = out
+    if _w4_check("quantize_w4", q, scale, None, group) != (N, K):
+        raise KatzError("quantize_w4: out does not match w %s" % (tuple(w.shape),))
+    _same_device(q, w.device, "out")
+    if N:
+        _call_on(w.device, "katz_quantize_w4_f16", w.data_ptr(), max(w.stride(0), K), q.data_ptr(), scale.data_ptr(), N, K, group)
+    return q, scale
+
+
+def dequantize_w4(q, scale, zero=None, group=64, out=None):
+    """4-bit weights -> fp16 [N, K] = scale * (code - zero), rounded once. `zero`: uint8 of scale's shape, 0..15 (None: 8)."""
+    N, K = _w4_check("dequantize_w4", q, scale, zero, group)
+    if out is None:
+        out = torch.empty((N, K), dtype=torch.float16, device=q.device)
+    _same_device(_f16(out, "out"), q.device, "out")
+    if not _rows_ok(out, N, K) or not _al16(out) or (N > 1 and out.stride(0) % 8):
+        raise KatzError("dequantize_w4: out must be [N, K] with unit column stride and 16-byte aligned rows")
+    if N:
+        _call_on(q.device, "katz_dequantize_w4_f16", q.data_ptr(), scale.data_ptr(), zero.data_ptr() if zero is not None else None,
+                 out.data_ptr(), max(out.stride(0), K), N, K, group)
+    return out
+
+
+def linear_w4(x, q, scale, zero=None, group=64, bias=None, residual=None, act=ACT_NONE, out=None, out_scale=1.0):
+    """`linear` with 4-bit weights (the format of quantize_w4, optionally with zero points): out[M,N] = x[M,K] @ w[N,K]^T
+    (+bias) -> act -> (+residual) * out_scale, fp32 accumulation, one rounding. Any M (0 included) and N.
+    `x`, `residual`, `out` may be row-strided 2-D views (unit column stride); `out` may be `residual`. Scales of 2^-23 to 64
+    are covered: the weights of larger ones overflow fp16 to infinity, those of smaller ones lose bits."""
+    _f16(x, "x")
+    N, K = _w4_check("linear_w4", q, scale, zero, group)
+    dev = x.device
+    _same_device(q, dev, "q")
+    M = x.shape[0]
+    if not _rows_ok(x, M, K):
+        raise KatzError("linear_w4: x must be [M, %d] with unit column stride (got %s, strides %s)" % (K, tuple(x.shape), x.stride()))
+    if act not in (ACT_NONE, ACT_SILU):
+        raise KatzError("linear_w4: unknown activation %r" % (act,))
+    if out is None:
+        out = torch.empty((M, N), dtype=torch.float16, device=dev)
+    else:
+        _same_device(_f16(out, "out"), dev, "out")
+        if not _rows_ok(out, M, N) or (M and N and out.data_ptr() == x.data_ptr()):
+            raise KatzError("linear_w4: bad out")
+    if bias is not None:
+        _same_device(_f16(bias, "bias"), dev, "bias")
+        if bias.shape != (N,) or not bias.is_contiguous():
+            raise KatzError("linear_w4: bias must be a contiguous [N] tensor")
+    if residual is not None:
+        _same_device(_f16(residual, "residual"), dev, "residual")
+        if not _rows_ok(residual, M, N) or (residual.data_ptr() == out.data_ptr() and M > 1 and residual.stride(0) != out.stride(0)):
+            raise KatzError("linear_w4: bad residual")
+    if M and N:
+        _call_on(dev, "katz_linear_w4_f16", x.data_ptr(), max(x.stride(0), K), q.data_ptr(), scale.data_ptr(),
+                 zero.data_ptr() if zero is not None else None, group, out.data_ptr(), max(out.stride(0), N), M, N, K,
+                 bias.data_ptr() if bias is not None else None, residual.data_ptr() if residual is not None else None,
+                 max(residual.stride(0), N) if residual is not None else 0, act, float(out_scale))
+    return out
+
+
 def conv2d(x, w, bias=None, ksize=3, stride=1, pad=1, upsample=False, x2=None, rowvec=None, residual=None,
            act=ACT_NONE, out=None, out_scale=1.0, pad_h=None):
     """NHWC convolution. x: [B,Hs,Ws,C1] (+ optional x2 [B,Hs,Ws,C2] concatenated along channels); w: [Cout,k,k,C1+C2].
@@ -319,6 +437,121 @@ def layer_norm(x, gamma, beta, eps=1e-5, out=None):
         out = torch.empty_like(x)
     call("katz_layer_norm_f16", _p(x), _p(out), _p(gamma), _p(beta), rows, C, float(eps), _stream())
     return out
+
+
+class Norm:
+    """A norm of `residual_norm`: kind "layer" ((v - mean) / sqrt(var + eps)) or "rms" (v / sqrt(mean of v^2 + eps)), with optional
+    fp16 weight [C] and bias [C]."""
+
+    def __init__(self, kind, weight=None, bias=None, eps=1e-5):
+        if kind not in ("layer", "rms"):
+            raise KatzError('Norm: kind must be "layer" or "rms" (got %r)' % (kind,))
+        if not 0.0 <= float(eps) < float("inf"):
+            raise KatzError("Norm: eps must be finite and not negative (got %r)" % (eps,))
+        self.kind, self.weight, self.bias, self.eps = kind, weight, bias, float(eps)
+        self.code = _lib.NORM_LAYER if kind == "layer" else _lib.NORM_RMS
+
+
+def _row_strides(t, name, shape):
+    """(batch, token) strides of an activation [rows, C] or [B, S, C] of the given shape with unit channel stride."""
+    if t.shape != shape or (t.stride(-1) != 1 and shape[-1] != 1):
+        raise KatzError("residual_norm: %s must be %s with unit channel stride (got %s, strides %s)" % (name, tuple(shape), tuple(t.shape), t.stride()))
+    return (t.stride(0) if len(shape) == 3 and shape[0] > 1 else 0), (t.stride(-2) if shape[-2] > 1 else 0)
+
+
+def _written_rows(t, name, shape, dtype, device):
+    if t.dtype != dtype or t.device != device:
+        raise KatzError("residual_norm: %s must be a %s tensor on %s" % (name, dtype, device))
+    sb, ss = _row_strides(t, name, shape)
+    C, S = shape[-1], shape[-2]
+    if (S > 1 and ss < C) or (len(shape) == 3 and shape[0] > 1 and sb < (S - 1) * ss + C):
+        raise KatzError("residual_norm: the rows of %s overlap" % name)
+    return sb, ss
+
+
+def _vector_strides(t, name, shape, device):
+    """(batch, token) strides of a gate, scale or shift: [C], [B, C] ([rows, C] for a 2-D x) or [B, S, C], sizes of 1 broadcast."""
+    _same_device(_f16(t, name), device, name)
+    d, C = t.dim(), shape[-1]
+    if d == 0 or d > len(shape) or t.shape[-1] != C or (t.stride(-1) != 1 and C != 1):
+        raise KatzError("residual_norm: %s %s does not fit x %s (unit channel stride)" % (name, tuple(t.shape), tuple(shape)))
+    for i in range(d - 1):
+        if t.shape[i] != shape[i] and t.shape[i] != 1:
+            raise KatzError("residual_norm: %s %s does not fit x %s" % (name, tuple(t.shape), tuple(shape)))
+    st = [t.stride(i) if t.shape[i] != 1 else 0 for i in range(d - 1)]
+    if len(shape) == 2:
+        return 0, st[0] if st else 0
+    return (st + [0, 0])[:2]
+
+
+def residual_norm(x, y=None, gate=None, post=None, pre=None, scale=None, shift=None, residual_scale=1.0, out=None, normed=None):
+    """The norms after and before a block with its gate and the residual scale between them, in one kernel:
+    `h = residual_scale * x + gate * post(y)`, `z = pre(h) * (1 + scale) + shift`; returns (h, z).
+    x: [rows, C] or [B, S, C], the residual stream, fp16 or fp32; y: the block's output, fp16, x's shape; C <= 16384.
+    post, pre: Norm or None. gate, scale, shift: fp16, per channel [C], per sample [B, C], per token [B, S, C] (a 2-D x: [C]
+    or [rows, C]); sizes of 1 broadcast and any may be a view into a wider row. h has x's type, z is fp16 and None without
+    `pre`; both are rounded once, z from the unrounded h. Without y, h is residual_scale * x (x itself where that is 1 and no
+    `out` is given). `out` (for h) may be x, `normed` (for z) may be y; all last strides are 1."""
+    if not x.is_cuda or x.dtype not in (torch.float16, torch.float32):
+        raise KatzError("x must be a CUDA fp16 or fp32 tensor (got %s on %s)" % (x.dtype, x.device))
+    shape, dev = x.shape, x.device
+    if len(shape) not in (2, 3) or not 0 < shape[-1] <= _lib.RESIDUAL_NORM_MAX_C:
+        raise KatzError("residual_norm: x must be [rows, C] or [B, S, C] with 1 <= C <= %d (got %s)" % (_lib.RESIDUAL_NORM_MAX_C, tuple(shape)))
+    if y is None and (gate is not None or post is not None):
+        raise KatzError("residual_norm: gate and post need y")
+    if pre is None and (scale is not None or shift is not None or normed is not None):
+        raise KatzError("residual_norm: scale, shift and normed need pre")
+    if y is None and pre is None:
+        raise KatzError("residual_norm: neither y nor pre: nothing to compute")
+    a = _lib.ResidualNormArgs()
+    a.x = x.data_ptr()
+    a.x_sb, a.x_ss = _row_strides(x, "x", shape)
+    a.B, a.S, a.C = (shape[0] if len(shape) == 3 else 1), shape[-2], shape[-1]
+    a.x_dtype = _lib.KATZ_DTYPE_F16 if x.dtype == torch.float16 else _lib.KATZ_DTYPE_F32
+    a.residual_scale = residual_scale
+    if y is not None:
+        _same_device(_f16(y, "y"), dev, "y")
+        a.y = y.data_ptr()
+        a.y_sb, a.y_ss = _row_strides(y, "y", shape)
+    if gate is not None:
+        a.gate = gate.data_ptr()
+        a.gate_sb, a.gate_ss = _vector_strides(gate, "gate", shape, dev)
+    if scale is not None:
+        a.scale = scale.data_ptr()
+        a.scale_sb, a.scale_ss = _vector_strides(scale, "scale", shape, dev)
+    if shift is not None:
+        a.shift = shift.data_ptr()
+        a.shift_sb, a.shift_ss = _vector_strides(shift, "shift", shape, dev)
+    for side, norm in (("post", post), ("pre", pre)):
+        if norm is None:
+            continue
+        for part in ("weight", "bias"):
+            v = getattr(norm, part)
+            if v is not None:
+                _same_device(_f16(v, "%s.%s" % (side, part)), dev, "%s.%s" % (side, part))
+                if v.shape != (shape[-1],) or not v.is_contiguous():
+                    raise KatzError("residual_norm: %s.%s must be a contiguous [C] tensor" % (side, part))
+                setattr(a, "%s_%s" % (side, part), v.data_ptr())
+    if post is not None:
+        a.post_kind, a.post_eps = post.code, post.eps
+    h, z = out, None
+    if out is None:
+        h = x if y is None and residual_scale == 1.0 else torch.empty(shape, dtype=x.dtype, device=dev)
+    if h is not x or out is not None:
+        a.h = h.data_ptr()
+        a.h_sb, a.h_ss = _written_rows(h, "out", shape, x.dtype, dev)
+    if pre is not None:
+        a.pre_kind, a.pre_eps = pre.code, pre.eps
+        z = torch.empty(shape, dtype=torch.float16, device=dev) if normed is None else normed
+        a.z = z.data_ptr()
+        a.z_sb, a.z_ss = _written_rows(z, "normed", shape, torch.float16, dev)
+    if x.numel() == 0:
+        return h, z
+    if (a.h and (a.h == a.y or a.h == a.z or (a.h == a.x and (a.h_sb, a.h_ss) != (a.x_sb, a.x_ss)))) \
+            or (a.z and (a.z == a.x or (a.z == a.y and (a.z_sb, a.z_ss) != (a.y_sb, a.y_ss)))):
+        raise KatzError("residual_norm: out may only be x, normed may only be y, with the same strides")
+    _call_on(dev, "katz_residual_norm_f16", ctypes.byref(a))
+    return h, z
 
 
 def geglu_erf(hg, out=None):
