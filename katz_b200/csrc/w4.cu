@@ -129,28 +129,6 @@ __global__ void __launch_bounds__(256) dequantize_w4_kernel(const unsigned char*
 // gives are matched by pairing x with a byte permute. The warps' sums meet in shared memory, added in warp order.
 constexpr int W4_ROWS_WARPS = 8;
 
-struct W4Params {
-    const __half* x;
-    const unsigned char* q;
-    const unsigned short* scale;
-    const unsigned char* zero;
-    const __half* bias;
-    const __half* residual;
-    __half* out;
-    long long ldx, ldo, ldr;
-    int M, N, K, J, group_shift;
-    int act;
-    float out_scale;
-};
-
-__device__ __forceinline__ float w4_epilogue(const W4Params& p, float acc, int m, int n) {
-    float v = acc * OPERAND_UNSCALE;
-    if (p.bias) v += __half2float(p.bias[n]);
-    if (p.act == KATZ_ACT_SILU) v = silu_f(v);
-    if (p.residual) v += __half2float(p.residual[m * p.ldr + n]);
-    return v * p.out_scale;
-}
-
 template <int MT, int RT, bool XALIGNED>
 __global__ void __launch_bounds__(W4_ROWS_WARPS * 32) linear_w4_rows_kernel(const W4Params p) {
     __shared__ float red[W4_ROWS_WARPS][8 * MT][16 * RT + 4];
@@ -298,6 +276,7 @@ extern "C" int katz_linear_w4_f16(const void* x, long long ldx, const void* q, c
     KATZ_CHECK_ARG(ceil_div(M, 32) <= 65535, KATZ_ESIZE);
     const bool xaligned = aligned16(x) && (M == 1 || ldx % 8 == 0);
     cudaStream_t st = (cudaStream_t)stream;
+    if (M > 16 && xaligned && K >= W4_TC05_MIN_K) return linear_w4_tc05(p, st);
     if (M <= 8) launch_rows<1, 1>(p, xaligned, st);
     else if (M <= 16) launch_rows<2, 1>(p, xaligned, st);
     else launch_rows<4, 2>(p, xaligned, st);

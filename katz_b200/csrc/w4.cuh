@@ -63,4 +63,31 @@ __device__ __forceinline__ void weights8(uint32_t w, const Group& g, uint32_t* o
 }
 
 }  // namespace w4
+
+struct W4Params {
+    const __half* x;
+    const unsigned char* q;
+    const unsigned short* scale;
+    const unsigned char* zero;
+    const __half* bias;
+    const __half* residual;
+    __half* out;
+    long long ldx, ldo, ldr;
+    int M, N, K, J, group_shift;
+    int act;
+    float out_scale;
+};
+
+__device__ __forceinline__ float w4_epilogue(const W4Params& p, float acc, int m, int n) {
+    float v = acc * w4::OPERAND_UNSCALE;
+    if (p.bias) v += __half2float(p.bias[n]);
+    if (p.act == KATZ_ACT_SILU) v = silu_f(v);
+    if (p.residual) v += __half2float(p.residual[m * p.ldr + n]);
+    return v * p.out_scale;
+}
+
+// The product for more rows on the tcgen05 path (w4_tc05.cu): p.x 16-byte aligned with ldx % 8 == 0, K >= W4_TC05_MIN_K.
+constexpr int W4_TC05_MIN_K = 128;
+int linear_w4_tc05(const W4Params& p, cudaStream_t st);
+
 }  // namespace katz

@@ -1,0 +1,562 @@
+// Products with 4-bit weights (w4.cuh has the format) on the tcgen05 tensor path, for more rows than the few of w4.cu:
+// out[M, N] = (act(x W^T + bias) + residual) * out_scale.
+//
+// The WEIGHT rows are the 128 rows of the MMA and the rows of x its columns (BT of them, any multiple of 16 up to 256), so a
+// few dozen rows of x waste nothing. The weights never exist in memory as fp16: warps unpack them in registers and write
+// them to TENSOR MEMORY, from where the MMA reads its A operand; shared memory carries the 4-bit codes and x only. One
+// persistent CTA per SM, sixteen warps:
+//   * warps 0-7 unpack: a warp owns 32 weight rows (its TMEM lane quarter, one row per thread) and 32 of a k-step's 64 k:
+//     16 bytes of codes from shared memory, 16 fp16 pairs to TMEM (tcgen05.st), a ring of 32-column stages;
+//   * warps 8-11: epilogue, one weight row per thread; for each row of x a warp stores 32 consecutive outputs (64 bytes);
+//   * warp 12: TMA loads of x (64 k per stage, 128-byte swizzle); warp 14: TMA loads of codes (128 k per stage, 64-byte
+//     swizzle), a ring of its own so that the HBM stream of codes runs ahead of what x's ring holds;
+//   * warp 15: scales and zero points of 512 k at a time, gathered into shared memory as fp16 (64 * scale);
+//   * warp 13: tcgen05.mma, D[128 x BT] += A[TMEM] B[x].
+// CTA pairs (PAIR): the MMA covers 256 weight rows, 128 from each CTA's tensor memory, and each CTA loads half of x's tile:
+// per k-step an SM then fetches BT * 64 + 4096 bytes instead of BT * 128 + 4096, where L2 was the bound.
+//
+// Every mbarrier wait is bounded (tc05.cuh): on a time-out the CTA records a status word, stops storing, frees its TMEM and
+// returns; the host reads the word with katz_tc05_status().
+#include "tc05.cuh"
+#include "w4.cuh"
+#include "katz_b200.h"
+
+namespace katz {
+
+using namespace tc05;
+using namespace w4;
+
+int* tc05_status_device_ptr();   // defined next to the status word (gemm_tc05.cu)
+
+constexpr int WT_THREADS = 768;
+constexpr int WT_GROUPS = 2, WT_GROUP_WARPS = 8;               // unpacking warps
+constexpr int WT_UNPACK_WARPS = WT_GROUPS * WT_GROUP_WARPS;
+constexpr int WT_EPILOGUE = WT_UNPACK_WARPS, WT_X = WT_EPILOGUE + 4, WT_MMA = WT_X + 1, WT_Q = WT_X + 2;   // first warp of each role
+constexpr int WT_XS = 8, WT_QS = 8, WT_AS = 8, WT_SS = 3;      // most stages of each ring
+constexpr int WT_Q_BYTES = 128 * 64;                           // 128 rows x 128 k of codes
+constexpr int WT_S_ROWS = 512 / 32;                            // groups of a scale block at most
+constexpr int WT_SCALE_BYTES = WT_S_ROWS * 128 * 2, WT_ZERO_BYTES = WT_S_ROWS * 128;
+constexpr int WT_TMEM_COLS = 512;
+constexpr int WT_BARS = 2 * (WT_XS + WT_QS + WT_AS + WT_SS + 2);
+constexpr int WT_FIXED_SMEM = WT_SS * (WT_SCALE_BYTES + WT_ZERO_BYTES) + WT_BARS * 8 + 16 + 1024;
+constexpr int WT_MAX_SMEM = 232448;
+
+struct W4Tile {
+    int bt, acc_stride, n_acc;                 // columns of a tile (rows of x), of an accumulator buffer; buffers
+    int x_stages, q_stages, a_stages, x_bytes; // x_bytes: what this CTA loads per k-step
+    int m_tiles, n_tiles;                      // n_tiles: of 128 rows, of a pair's 256
+    int* status;
+};
+
+// One word (8 codes, k = 0..7) -> 64 * weight as four fp16 pairs in k order. Byte i of the word is copied into both halves;
+// the low half keeps its low four bits (1024 + code), the high half its high four (1024 + 16 code, times 1/16).
+__device__ __forceinline__ void weights8_in_order(uint32_t w, __half2 minus, __half2 scale, uint32_t* o) {
+    const __half2 mul = as_half2(0x2c003c00u);      // (1, 1/16)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t both = __byte_perm(w, 0, 0x4040 + 0x0101 * i);
+        const __half2 d = __hfma2(as_half2(and_or_1024<0x00f0000fu>(both)), mul, minus);
+        o[i] = as_u32(__hmul2(d, scale));
+    }
+}
+
+// position in a ring of `n` stages
+struct Ring {
+    uint32_t s = 0, phase = 0;
+    __device__ __forceinline__ void next(uint32_t n) {
+        if (++s == n) {
+            s = 0;
+            phase ^= 1;
+        }
+    }
+};
+
+template <bool PAIR>
+__global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __grid_constant__ CUtensorMap tmX,
+                                                                       const __grid_constant__ CUtensorMap tmQ, const W4Params p,
+                                                                       const W4Tile t) {
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    unsigned char* q_ring = smem + t.x_stages * t.x_bytes;
+    unsigned char* s_ring = q_ring + t.q_stages * WT_Q_BYTES;
+    unsigned char* z_ring = s_ring + WT_SS * WT_SCALE_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(z_ring + WT_SS * WT_ZERO_BYTES);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + WT_BARS);
+    const uint32_t x_full = smem_u32(bars), x_empty = x_full + 8 * WT_XS, q_full = x_empty + 8 * WT_XS, q_empty = q_full + 8 * WT_QS,
+                   a_full = q_empty + 8 * WT_QS, a_empty = a_full + 8 * WT_AS, s_full = a_empty + 8 * WT_AS,
+                   s_empty = s_full + 8 * WT_SS, acc_full = s_empty + 8 * WT_SS, acc_empty = acc_full + 16;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = PAIR ? cluster_ctarank() : 0;
+    constexpr int CTAS = PAIR ? 2 : 1;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < WT_XS; ++i) {
+            mbar_init(x_full + 8 * i, 1);
+            mbar_init(x_empty + 8 * i, 1);
+        }
+        for (int i = 0; i < WT_QS; ++i) {
+            mbar_init(q_full + 8 * i, 1);
+            mbar_init(q_empty + 8 * i, WT_GROUP_WARPS);
+        }
+        for (int i = 0; i < WT_AS; ++i) {
+            mbar_init(a_full + 8 * i, WT_GROUP_WARPS * CTAS);
+            mbar_init(a_empty + 8 * i, 1);
+        }
+        for (int i = 0; i < WT_SS; ++i) {
+            mbar_init(s_full + 8 * i, 1);
+            mbar_init(s_empty + 8 * i, WT_UNPACK_WARPS);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(acc_full + 8 * i, 1);
+            mbar_init(acc_empty + 8 * i, 4 * CTAS);
+        }
+        fence_barrier_init();
+        tma_prefetch_desc(&tmX);
+        tma_prefetch_desc(&tmQ);
+    }
+    if (warp == WT_MMA) {
+        if (PAIR) {
+            tmem_alloc_pair(smem_u32(tmem_slot), WT_TMEM_COLS);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(smem_u32(tmem_slot), WT_TMEM_COLS);
+            tmem_relinquish();
+        }
+    }
+    fence_before_sync();
+    __syncthreads();
+    if (PAIR) cluster_sync_all();      // the peer's barriers are initialised before anything signals them
+    fence_after_sync();
+    const uint32_t tmem_base = *tmem_slot;
+    const uint32_t a_base = tmem_base + t.n_acc * t.acc_stride;
+
+    const int steps = (p.K + 63) >> 6, units = (p.K + 127) >> 7;      // of 64 k (x), of 128 k (codes, A)
+    const int total = t.m_tiles * t.n_tiles;
+    const int item0 = (int)blockIdx.x / CTAS, item_stride = (int)gridDim.x / CTAS;
+    auto rows_of = [&](int tile, int& m0, int& n0) {      // weight rows fastest: CTAs at work at one time share x
+        const int mt = tile / t.n_tiles;
+        m0 = mt * t.bt;
+        n0 = (tile - mt * t.n_tiles) * 128 * CTAS + 128 * (int)rank;
+    };
+    // Nothing above touches global memory; every role waits for the kernels this launch depends on before it goes on (those
+    // that read none as well: their bounded waits must not run out while a predecessor still runs).
+    pdl_wait();
+    pdl_launch_dependents();
+
+    if (warp < WT_UNPACK_WARPS) {
+        // ---------------------------------------------------------------------------------------- unpack
+        const int quarter = warp & 3, h = (warp >> 2) & 1;
+        const uint32_t group = warp / WT_GROUP_WARPS;
+        const int row = quarter * 32 + lane;
+        const uint32_t a_mine = a_base + ((uint32_t)(quarter * 32) << 16) + 32 * h;
+        const uint32_t swz = (uint32_t)((row >> 1) & 3);
+        const uint32_t q_mine0 = row * 64 + (((uint32_t)(2 * h) ^ swz) << 4), q_mine1 = row * 64 + (((uint32_t)(2 * h + 1) ^ swz) << 4);
+        Ring q, a, sc;
+        uint32_t turn = 0;
+        bool ok = true;
+        for (int tile = item0; tile < total && ok; tile += item_stride) {
+            for (int u = 0; u < units; ++u) {
+                // both groups wait for every scale block, so that neither can be a whole ring ahead of the other
+                if ((u & 3) == 0) ok = mbar_wait(s_full + 8 * sc.s, sc.phase);
+                if (turn == group) {
+                    ok = ok && mbar_wait(q_full + 8 * q.s, q.phase);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    const unsigned char* codes = q_ring + q.s * WT_Q_BYTES;
+                    const uint4 v0 = *reinterpret_cast<const uint4*>(codes + q_mine0), v1 = *reinterpret_cast<const uint4*>(codes + q_mine1);
+                    const int k = (u & 3) * 128 + 64 * h, j0 = (k >> p.group_shift) * 128 + row, j1 = ((k + 32) >> p.group_shift) * 128 + row;
+                    const __half* scales = reinterpret_cast<const __half*>(s_ring + sc.s * WT_SCALE_BYTES);
+                    const __half2 scale0 = __half2half2(scales[j0]), scale1 = __half2half2(scales[j1]);
+                    uint32_t minus0 = 0xd480e408u, minus1 = minus0;      // (-(1024 + 8), -(64 + 8))
+                    if (p.zero) {
+                        const unsigned char* zeros = z_ring + sc.s * WT_ZERO_BYTES;
+                        minus0 = 0xd400e400u + 0x00100001u * zeros[j0];
+                        minus1 = 0xd400e400u + 0x00100001u * zeros[j1];
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(q_empty + 8 * q.s);
+                    uint32_t w[32];
+                    weights8_in_order(v0.x, as_half2(minus0), scale0, w);
+                    weights8_in_order(v0.y, as_half2(minus0), scale0, w + 4);
+                    weights8_in_order(v0.z, as_half2(minus0), scale0, w + 8);
+                    weights8_in_order(v0.w, as_half2(minus0), scale0, w + 12);
+                    weights8_in_order(v1.x, as_half2(minus1), scale1, w + 16);
+                    weights8_in_order(v1.y, as_half2(minus1), scale1, w + 20);
+                    weights8_in_order(v1.z, as_half2(minus1), scale1, w + 24);
+                    weights8_in_order(v1.w, as_half2(minus1), scale1, w + 28);
+                    ok = mbar_wait(a_empty + 8 * a.s, a.phase ^ 1);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    fence_after_sync();
+                    tmem_st_32x32(a_mine + 64 * a.s, w);
+                    tmem_st_wait();
+                    fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (PAIR) mbar_arrive_cluster_tmem(mapa_shared(a_full + 8 * a.s, 0));      // the leader's MMA thread waits for both CTAs
+                        else mbar_arrive(a_full + 8 * a.s);
+                    }
+                }
+                if ((u & 3) == 3 || u == units - 1) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(s_empty + 8 * sc.s);
+                    sc.next(WT_SS);
+                }
+                q.next(t.q_stages);
+                a.next(t.a_stages);
+                if (++turn == WT_GROUPS) turn = 0;
+            }
+        }
+        if (!ok && lane == 0) atomicCAS(t.status, 0, 21);
+    } else if (warp < WT_X) {
+        // ---------------------------------------------------------------------------------------- epilogue
+        const int quarter = warp & 3;
+        Ring acc;
+        bool ok = true;
+        for (int tile = item0; tile < total; tile += item_stride) {
+            int m0, n0;
+            rows_of(tile, m0, n0);
+            const int n = n0 + quarter * 32 + lane;
+            const bool in = n < p.N;
+            const float bias = p.bias && in ? __half2float(p.bias[n]) : 0.f;
+            ok = mbar_wait(acc_full + 8 * acc.s, acc.phase);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            fence_after_sync();
+            const uint32_t tacc = tmem_base + acc.s * t.acc_stride + ((uint32_t)(quarter * 32) << 16);
+            const int rows = min(t.bt, p.M - m0);
+            for (int c = 0; c < rows; c += 16) {
+                uint32_t r[16];
+                tmem_ld_32x16(tacc + c, r);
+                const int left = rows - c;
+                unsigned short res[16];
+                if (p.residual) {
+                    const __half* src = p.residual + (long long)(m0 + c) * p.ldr + n;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) res[e] = in && e < left ? *reinterpret_cast<const unsigned short*>(src + e * p.ldr) : 0;
+                }
+                tmem_ld_wait();
+                __half* dst = p.out + (long long)(m0 + c) * p.ldo + n;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    float v = fmaf(__uint_as_float(r[e]), OPERAND_UNSCALE, bias);
+                    if (p.act == KATZ_ACT_SILU) v = silu_f(v);
+                    if (p.residual) v += __half2float(__ushort_as_half(res[e]));
+                    if (in && e < left) dst[e * p.ldo] = __float2half_rn(v * p.out_scale);
+                }
+            }
+            fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+                if (PAIR) mbar_arrive_cluster_tmem(mapa_shared(acc_empty + 8 * acc.s, 0));
+                else mbar_arrive(acc_empty + 8 * acc.s);
+            }
+            acc.next(t.n_acc);
+        }
+        if (!ok && lane == 0) atomicCAS(t.status, 0, 22);
+    } else if (warp == WT_X) {
+        // ---------------------------------------------------------------------------------------- x
+        if (elect_one()) {
+            Ring x;
+            uint32_t issued = 0;
+            bool ok = true;
+            for (int tile = item0; tile < total && ok; tile += item_stride) {
+                int m0, n0;
+                rows_of(tile, m0, n0);
+                for (int s = 0; s < steps; ++s) {
+                    if (!mbar_wait(x_empty + 8 * x.s, x.phase ^ 1)) { ok = false; break; }
+                    const uint32_t dst = smem_u32(smem + x.s * t.x_bytes);
+                    if (PAIR) {
+                        // both CTAs' bytes are counted on the leader's barrier, which the leader arms for both
+                        if (rank == 0) mbar_expect_tx(x_full + 8 * x.s, 2 * t.x_bytes);
+                        tma_load_2d_pair(dst, &tmX, s * 64, m0 + (int)rank * (t.bt / 2), mapa_shared(x_full + 8 * x.s, 0));
+                    } else {
+                        mbar_expect_tx(x_full + 8 * x.s, t.x_bytes);
+                        tma_load_2d(dst, &tmX, s * 64, m0, x_full + 8 * x.s);
+                    }
+                    ++issued;
+                    x.next(t.x_stages);
+                }
+            }
+            if (!ok) {
+                atomicCAS(t.status, 0, 23);
+                // copies in flight land before the CTA's shared memory is released (a pair's second CTA waits for the first
+                // in the cluster barrier of the teardown: its copies are counted on the leader's barriers)
+                if (rank == 0) {
+                    const uint32_t n = t.x_stages, first = issued > n ? issued - n : 0;
+                    for (uint32_t i = first; i < issued; ++i) mbar_wait(x_full + 8 * (i % n), (i / n) & 1);
+                }
+            }
+        }
+    } else if (warp == WT_MMA) {
+        // ---------------------------------------------------------------------------------------- MMA
+        if (rank == 0 && elect_one()) {
+            const uint32_t idesc = idesc_f16(PAIR ? 256 : 128, t.bt);
+            Ring x, a, acc;
+            bool ok = true;
+            for (int tile = item0; tile < total && ok; tile += item_stride) {
+                if (!mbar_wait(acc_empty + 8 * acc.s, acc.phase ^ 1)) { ok = false; break; }
+                fence_after_sync();
+                const uint32_t tacc = tmem_base + acc.s * t.acc_stride;
+                for (int s = 0; s < steps; ++s) {
+                    if ((s & 1) == 0 && !mbar_wait(a_full + 8 * a.s, a.phase)) { ok = false; break; }
+                    if (!mbar_wait(x_full + 8 * x.s, x.phase)) { ok = false; break; }
+                    fence_after_sync();
+                    const uint64_t bd = smem_desc_sw128(smem_u32(smem + x.s * t.x_bytes));
+                    const uint32_t ta = a_base + 64 * a.s + 32 * (s & 1);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        if (PAIR) umma_f16_ta_pair(tacc, ta + 8 * k, bd + 2 * k, idesc, (s | k) != 0);
+                        else umma_f16_ta(tacc, ta + 8 * k, bd + 2 * k, idesc, (s | k) != 0);
+                    }
+                    if (PAIR) umma_commit_pair(x_empty + 8 * x.s, 3);
+                    else umma_commit(x_empty + 8 * x.s);
+                    x.next(t.x_stages);
+                    if ((s & 1) == 1 || s == steps - 1) {
+                        if (PAIR) umma_commit_pair(a_empty + 8 * a.s, 3);
+                        else umma_commit(a_empty + 8 * a.s);
+                        a.next(t.a_stages);
+                    }
+                }
+                if (ok) {
+                    if (PAIR) umma_commit_pair(acc_full + 8 * acc.s, 3);
+                    else umma_commit(acc_full + 8 * acc.s);
+                }
+                acc.next(t.n_acc);
+            }
+            if (!ok) atomicCAS(t.status, 0, 24);
+        }
+    } else if (warp == WT_Q) {
+        // ---------------------------------------------------------------------------------------- codes
+        if (elect_one()) {
+            Ring q;
+            uint32_t issued = 0;
+            bool ok = true;
+            for (int tile = item0; tile < total && ok; tile += item_stride) {
+                int m0, n0;
+                rows_of(tile, m0, n0);
+                for (int s = 0; s < steps; s += 2) {
+                    if (!mbar_wait(q_empty + 8 * q.s, q.phase ^ 1)) { ok = false; break; }
+                    mbar_expect_tx(q_full + 8 * q.s, WT_Q_BYTES);
+                    tma_load_2d(smem_u32(q_ring + q.s * WT_Q_BYTES), &tmQ, s * 32, n0, q_full + 8 * q.s);
+                    ++issued;
+                    q.next(t.q_stages);
+                }
+            }
+            if (!ok) {
+                atomicCAS(t.status, 0, 25);
+                const uint32_t n = t.q_stages, first = issued > n ? issued - n : 0;
+                for (uint32_t i = first; i < issued; ++i) mbar_wait(q_full + 8 * (i % n), (i / n) & 1);
+            }
+        }
+    } else {
+        // ---------------------------------------------------------------------------------------- scales, zero points
+        Ring sc;
+        bool ok = true;
+        const int per_block = 512 >> p.group_shift;
+        const bool by_four = (p.J & 3) == 0 && ((uintptr_t)p.scale & 7) == 0;
+        for (int tile = item0; tile < total && ok; tile += item_stride) {
+            int m0, n0;
+            rows_of(tile, m0, n0);
+            for (int j0 = 0; j0 < p.J; j0 += per_block) {
+                ok = mbar_wait(s_empty + 8 * sc.s, sc.phase ^ 1);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                __half* dst = reinterpret_cast<__half*>(s_ring + sc.s * WT_SCALE_BYTES);
+                unsigned char* zdst = z_ring + sc.s * WT_ZERO_BYTES;
+                // groups past the last and rows past the last get zeros: their weights are zeros
+                // (every load of a batch is requested before the first is used: one round trip a batch, not one a load)
+                if (by_four) {
+                    for (int b = 0; b < per_block; b += 8) {      // item i: groups 4 (i / 4) .. + 3 of 32 rows
+                        uint2 v[8];
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) {
+                            const int i = b + u, n = n0 + lane + 32 * (i & 3), jj = i & ~3;
+                            v[u] = make_uint2(0, 0);
+                            if (i < per_block && n < p.N && j0 + jj < p.J) v[u] = __ldg(reinterpret_cast<const uint2*>(p.scale + (size_t)n * p.J + j0 + jj));
+                        }
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) {
+                            const int i = b + u;
+                            if (i >= per_block) break;
+                            __half* d = dst + (i & ~3) * 128 + lane + 32 * (i & 3);
+                            d[0] = __float2half_rn(__uint_as_float(v[u].x << 16) * OPERAND_SCALE);
+                            d[128] = __float2half_rn(__uint_as_float(v[u].x & 0xffff0000u) * OPERAND_SCALE);
+                            d[256] = __float2half_rn(__uint_as_float(v[u].y << 16) * OPERAND_SCALE);
+                            d[384] = __float2half_rn(__uint_as_float(v[u].y & 0xffff0000u) * OPERAND_SCALE);
+                        }
+                    }
+                } else {
+                    for (int b = 0; b < 4 * per_block; b += 16) {      // item i: group i / 4 of 32 rows
+                        unsigned short v[16];
+#pragma unroll
+                        for (int u = 0; u < 16; ++u) {
+                            const int i = b + u, n = n0 + lane + 32 * (i & 3), jj = i >> 2;
+                            v[u] = n < p.N && j0 + jj < p.J ? __ldg(p.scale + (size_t)n * p.J + j0 + jj) : (unsigned short)0;
+                        }
+#pragma unroll
+                        for (int u = 0; u < 16; ++u) {
+                            const int i = b + u;
+                            dst[(i >> 2) * 128 + lane + 32 * (i & 3)] = __float2half_rn(bf16_bits_to_float(v[u]) * OPERAND_SCALE);
+                        }
+                    }
+                }
+                if (p.zero) {
+                    for (int b = 0; b < 4 * per_block; b += 16) {
+                        unsigned char v[16];
+#pragma unroll
+                        for (int u = 0; u < 16; ++u) {
+                            const int i = b + u, n = n0 + lane + 32 * (i & 3), jj = i >> 2;
+                            v[u] = n < p.N && j0 + jj < p.J ? __ldg(p.zero + (size_t)n * p.J + j0 + jj) : (unsigned char)0;
+                        }
+#pragma unroll
+                        for (int u = 0; u < 16; ++u) {
+                            const int i = b + u;
+                            zdst[(i >> 2) * 128 + lane + 32 * (i & 3)] = v[u];
+                        }
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_full + 8 * sc.s);
+                sc.next(WT_SS);
+            }
+        }
+        if (!ok && lane == 0) atomicCAS(t.status, 0, 26);
+    }
+    // -------------------------------------------------------------------------------------------- teardown
+    __syncwarp();
+    fence_before_sync();
+    __syncthreads();
+    if (PAIR) cluster_sync_all();      // neither CTA leaves (or frees TMEM) while the other may still signal it or read its tiles
+    if (warp == WT_MMA) {
+        fence_after_sync();
+        if (PAIR) tmem_dealloc_pair(tmem_base, WT_TMEM_COLS);
+        else tmem_dealloc(tmem_base, WT_TMEM_COLS);
+    }
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------------
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiledFn get_encode() {
+    static const EncodeTiledFn fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult qres;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &qres) != cudaSuccess ||
+            qres != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<EncodeTiledFn>(f);
+    }();
+    return fn;
+}
+
+static int encode_rows(CUtensorMap* map, CUtensorMapDataType type, CUtensorMapSwizzle swizzle, const void* base, uint64_t inner,
+                       uint64_t outer, uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer) {
+    EncodeTiledFn enc = get_encode();
+    if (!enc) return KATZ_ENOTREADY;
+    cuuint64_t dims[2] = {inner, outer};
+    cuuint64_t strides[1] = {row_bytes};
+    cuuint32_t box[2] = {box_inner, box_outer};
+    cuuint32_t es[2] = {1, 1};
+    CUresult r = enc(map, type, 2, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : KATZ_EINVAL;
+}
+
+struct W4Device {
+    int sms, pairs;      // CTAs and CTA pairs that are resident at once
+    bool ready;
+};
+
+static int device_limits(W4Device& out) {
+    static W4Device cached[KATZ_MAX_DEVICES] = {};
+    W4Device& d = cached[current_device_index()];
+    if (!d.ready) {
+        int dev = 0, sms = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(linear_w4_tc05_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, WT_MAX_SMEM);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(linear_w4_tc05_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, WT_MAX_SMEM);
+        if (e != cudaSuccess) return (int)e;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(2 * sms);
+        cfg.blockDim = dim3(WT_THREADS);
+        cfg.dynamicSmemBytes = WT_MAX_SMEM;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = 2;
+        at[0].val.clusterDim.y = 1;
+        at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        int pairs = 0;
+        e = cudaOccupancyMaxActiveClusters(&pairs, linear_w4_tc05_kernel<true>, &cfg);
+        if (e != cudaSuccess || pairs <= 0) return e != cudaSuccess ? (int)e : KATZ_ENOTREADY;
+        d.sms = sms;
+        d.pairs = pairs;
+        d.ready = true;
+    }
+    out = d;
+    return 0;
+}
+
+int linear_w4_tc05(const W4Params& p, cudaStream_t st) {
+    W4Device dev;
+    int rc = device_limits(dev);
+    if (rc) return rc;
+    // Tile choice: the least modelled time over the number of tiles along M, alone or in pairs. Per k-step of 64 a CTA
+    // spends 2 BT cycles in the tensor pipe, its loads at about 48 bytes a cycle from L2, and about 190 cycles of unpacking.
+    const int steps = ceil_div(p.K, 64);
+    W4Tile t{};
+    bool pair = false;
+    double best = 1e30;
+    const int min_tiles = ceil_div(p.M, 256);
+    for (int mt = min_tiles; mt <= min_tiles + 8; ++mt) {
+        const int bt = ceil_div(ceil_div(p.M, mt), 16) * 16;
+        const int m_tiles = ceil_div(p.M, bt);
+        for (int two = 0; two < 2; ++two) {
+            if (two && p.N <= 128) continue;
+            const int n_tiles = ceil_div(p.N, two ? 256 : 128), slots = two ? dev.pairs : dev.sms;
+            const int n_acc = bt <= 160 ? 2 : 1;      // three stages of 64 columns beside them
+            const long long waves = ceil_div_ll((long long)m_tiles * n_tiles, slots);
+            double step = 2.0 * bt, load = (bt * (two ? 64.0 : 128.0) + 4096.0) / 48.0;
+            if (load > step) step = load;
+            if (step < 190.0) step = 190.0;
+            const double drain = 600.0 + 8.0 * bt;
+            const double cost = waves * (steps * step + (n_acc == 1 ? drain : 100.0)) + drain;
+            if (cost < best) {
+                best = cost;
+                pair = two;
+                t.bt = bt;
+                t.m_tiles = m_tiles;
+                t.n_tiles = n_tiles;
+                t.n_acc = n_acc;
+            }
+        }
+    }
+    KATZ_CHECK_ARG((long long)t.m_tiles * t.n_tiles < (1ll << 30), KATZ_ESIZE);
+    t.acc_stride = ceil_div(t.bt, 32) * 32;
+    t.x_bytes = t.bt * (pair ? 64 : 128);
+    t.q_stages = t.x_bytes <= 16384 ? WT_QS : 5;
+    const int room = (WT_MAX_SMEM - WT_FIXED_SMEM - t.q_stages * WT_Q_BYTES) / t.x_bytes;
+    t.x_stages = room < WT_XS ? room : WT_XS;
+    const int cols = (WT_TMEM_COLS - t.n_acc * t.acc_stride) / 64;
+    t.a_stages = cols < WT_AS ? cols : WT_AS;
+    t.status = tc05_status_device_ptr();
+    if (!t.status) return KATZ_ENOTREADY;
+    CUtensorMap tx, tq;
+    rc = encode_rows(&tx, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, CU_TENSOR_MAP_SWIZZLE_128B, p.x, p.K, p.M, (uint64_t)p.ldx * 2, 64,
+                     pair ? t.bt / 2 : t.bt);
+    if (rc) return rc;
+    rc = encode_rows(&tq, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_64B, p.q, p.K / 2, p.N, p.K / 2, 64, 128);
+    if (rc) return rc;
+    const int smem = t.x_stages * t.x_bytes + t.q_stages * WT_Q_BYTES + WT_FIXED_SMEM;
+    const int tiles = t.m_tiles * t.n_tiles;
+    if (pair) launch_k_cluster(linear_w4_tc05_kernel<true>, 2 * (tiles < dev.pairs ? tiles : dev.pairs), WT_THREADS, smem, st, 2, tx, tq, p, t);
+    else launch_k_cluster(linear_w4_tc05_kernel<false>, tiles < dev.sms ? tiles : dev.sms, WT_THREADS, smem, st, 1, tx, tq, p, t);
+    KATZ_LAUNCH_RET();
+}
+
+}  // namespace katz
