@@ -17,6 +17,8 @@
 //
 // Every mbarrier wait is bounded (tc05.cuh): on a time-out the CTA records a status word, stops storing, frees its TMEM and
 // returns; the host reads the word with katz_tc05_status().
+#include <algorithm>
+
 #include "tc05.cuh"
 #include "w4.cuh"
 #include "katz_b200.h"
@@ -32,19 +34,20 @@ constexpr int WT_THREADS = 768;
 constexpr int WT_GROUPS = 2, WT_GROUP_WARPS = 8;               // unpacking warps
 constexpr int WT_UNPACK_WARPS = WT_GROUPS * WT_GROUP_WARPS;
 constexpr int WT_EPILOGUE = WT_UNPACK_WARPS, WT_X = WT_EPILOGUE + 4, WT_MMA = WT_X + 1, WT_Q = WT_X + 2;   // first warp of each role
-constexpr int WT_XS = 8, WT_QS = 8, WT_AS = 8, WT_SS = 3;      // most stages of each ring
+constexpr int WT_AS = 6, WT_QS = 8, WT_SS = 3;                 // most stages of each ring
 constexpr int WT_Q_BYTES = 128 * 64;                           // 128 rows x 128 k of codes
 constexpr int WT_S_ROWS = 512 / 32;                            // groups of a scale block at most
 constexpr int WT_SCALE_BYTES = WT_S_ROWS * 128 * 2, WT_ZERO_BYTES = WT_S_ROWS * 128;
 constexpr int WT_TMEM_COLS = 512;
-constexpr int WT_BARS = 2 * (WT_XS + WT_QS + WT_AS + WT_SS + 2);
+constexpr int WT_BARS = 2 * (WT_QS + WT_AS + WT_SS + 2);
 constexpr int WT_FIXED_SMEM = WT_SS * (WT_SCALE_BYTES + WT_ZERO_BYTES) + WT_BARS * 8 + 16 + 1024;
 constexpr int WT_MAX_SMEM = 232448;
 
 struct W4Tile {
     int bt, acc_stride, n_acc;                 // columns of a tile (rows of x), of an accumulator buffer; buffers
-    int x_stages, q_stages, a_stages, x_bytes; // x_bytes: what this CTA loads per k-step
+    int stages, q_stages, x_bytes;              // x_bytes: of x in a stage of this CTA (two boxes of 64 k)
     int m_tiles, n_tiles;                      // n_tiles: of 128 rows, of a pair's 256
+    bool in_pairs;                             // out (and residual) allow 4-byte accesses to (n, n + 1), n even
     int* status;
 };
 
@@ -69,6 +72,13 @@ struct Ring {
             phase ^= 1;
         }
     }
+    __device__ __forceinline__ void skip(uint32_t k, uint32_t n) {      // k <= n
+        s += k;
+        if (s >= n) {
+            s -= n;
+            phase ^= 1;
+        }
+    }
 };
 
 template <bool PAIR>
@@ -77,12 +87,12 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                                                                        const W4Tile t) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    unsigned char* q_ring = smem + t.x_stages * t.x_bytes;
+    unsigned char* q_ring = smem + t.stages * t.x_bytes;
     unsigned char* s_ring = q_ring + t.q_stages * WT_Q_BYTES;
     unsigned char* z_ring = s_ring + WT_SS * WT_SCALE_BYTES;
     uint64_t* bars = reinterpret_cast<uint64_t*>(z_ring + WT_SS * WT_ZERO_BYTES);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + WT_BARS);
-    const uint32_t x_full = smem_u32(bars), x_empty = x_full + 8 * WT_XS, q_full = x_empty + 8 * WT_XS, q_empty = q_full + 8 * WT_QS,
+    const uint32_t q_full = smem_u32(bars), q_empty = q_full + 8 * WT_QS,
                    a_full = q_empty + 8 * WT_QS, a_empty = a_full + 8 * WT_AS, s_full = a_empty + 8 * WT_AS,
                    s_empty = s_full + 8 * WT_SS, acc_full = s_empty + 8 * WT_SS, acc_empty = acc_full + 16;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -90,16 +100,12 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
     constexpr int CTAS = PAIR ? 2 : 1;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < WT_XS; ++i) {
-            mbar_init(x_full + 8 * i, 1);
-            mbar_init(x_empty + 8 * i, 1);
-        }
         for (int i = 0; i < WT_QS; ++i) {
             mbar_init(q_full + 8 * i, 1);
             mbar_init(q_empty + 8 * i, WT_GROUP_WARPS);
         }
         for (int i = 0; i < WT_AS; ++i) {
-            mbar_init(a_full + 8 * i, WT_GROUP_WARPS * CTAS);
+            mbar_init(a_full + 8 * i, WT_GROUP_WARPS * CTAS + 1);      // the unpacking warps and the bytes of x
             mbar_init(a_empty + 8 * i, 1);
         }
         for (int i = 0; i < WT_SS; ++i) {
@@ -130,7 +136,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
     const uint32_t tmem_base = *tmem_slot;
     const uint32_t a_base = tmem_base + t.n_acc * t.acc_stride;
 
-    const int steps = (p.K + 63) >> 6, units = (p.K + 127) >> 7;      // of 64 k (x), of 128 k (codes, A)
+    const int units = (p.K + 127) >> 7;      // stages of 128 k
     const int total = t.m_tiles * t.n_tiles;
     const int item0 = (int)blockIdx.x / CTAS, item_stride = (int)gridDim.x / CTAS;
     auto rows_of = [&](int tile, int& m0, int& n0) {      // weight rows fastest: CTAs at work at one time share x
@@ -151,19 +157,41 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
         const uint32_t a_mine = a_base + ((uint32_t)(quarter * 32) << 16) + 32 * h;
         const uint32_t swz = (uint32_t)((row >> 1) & 3);
         const uint32_t q_mine0 = row * 64 + (((uint32_t)(2 * h) ^ swz) << 4), q_mine1 = row * 64 + (((uint32_t)(2 * h + 1) ^ swz) << 4);
+        // The groups take turns over a tile's units. A warp has its next unit's codes in registers before it hands over the
+        // current one, and the two barriers it will need are polled once BEFORE the arithmetic, so that a barrier that has
+        // long been passed (the usual case) costs nothing: waiting where the data was needed, a unit took 1800 cycles for 330
+        // of arithmetic.
         Ring q, a, sc;
-        uint32_t turn = 0;
+        q.skip(group, t.q_stages);
+        a.skip(group, t.stages);
         bool ok = true;
+        uint4 v0, v1;
+        auto read_codes = [&]() {
+            const unsigned char* codes = q_ring + q.s * WT_Q_BYTES;
+            v0 = *reinterpret_cast<const uint4*>(codes + q_mine0);
+            v1 = *reinterpret_cast<const uint4*>(codes + q_mine1);
+        };
+        auto wait_all = [&](uint32_t bar, uint32_t phase) { return __all_sync(0xffffffffu, mbar_wait(bar, phase)); };
+        if ((int)group < units && item0 < total) {
+            ok = wait_all(q_full + 8 * q.s, q.phase);
+            if (ok) {
+                read_codes();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_empty + 8 * q.s);
+            }
+        }
         for (int tile = item0; tile < total && ok; tile += item_stride) {
-            for (int u = 0; u < units; ++u) {
+            for (int u0 = 0; u0 < units && ok; u0 += 4) {
                 // both groups wait for every scale block, so that neither can be a whole ring ahead of the other
-                if ((u & 3) == 0) ok = mbar_wait(s_full + 8 * sc.s, sc.phase);
-                if (turn == group) {
-                    ok = ok && mbar_wait(q_full + 8 * q.s, q.phase);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    const unsigned char* codes = q_ring + q.s * WT_Q_BYTES;
-                    const uint4 v0 = *reinterpret_cast<const uint4*>(codes + q_mine0), v1 = *reinterpret_cast<const uint4*>(codes + q_mine1);
+                ok = wait_all(s_full + 8 * sc.s, sc.phase);
+                const int u1 = min(u0 + 4, units);
+                for (int u = u0 + (int)group; u < u1 && ok; u += 2) {
+                    const uint32_t step = u + 2 < units ? 2 : units - u + group;      // to this group's next unit
+                    const bool more = u + 2 < units || tile + item_stride < total;
+                    const uint32_t a_bar = 8 * a.s, a_phase = a.phase ^ 1;
+                    q.skip(step, t.q_stages);
+                    const bool a_free = mbar_try_wait(a_empty + a_bar, a_phase);
+                    const bool q_there = more && mbar_try_wait(q_full + 8 * q.s, q.phase);
                     const int k = (u & 3) * 128 + 64 * h, j0 = (k >> p.group_shift) * 128 + row, j1 = ((k + 32) >> p.group_shift) * 128 + row;
                     const __half* scales = reinterpret_cast<const __half*>(s_ring + sc.s * WT_SCALE_BYTES);
                     const __half2 scale0 = __half2half2(scales[j0]), scale1 = __half2half2(scales[j1]);
@@ -173,8 +201,6 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                         minus0 = 0xd400e400u + 0x00100001u * zeros[j0];
                         minus1 = 0xd400e400u + 0x00100001u * zeros[j1];
                     }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(q_empty + 8 * q.s);
                     uint32_t w[32];
                     weights8_in_order(v0.x, as_half2(minus0), scale0, w);
                     weights8_in_order(v0.y, as_half2(minus0), scale0, w + 4);
@@ -184,27 +210,38 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                     weights8_in_order(v1.y, as_half2(minus1), scale1, w + 20);
                     weights8_in_order(v1.z, as_half2(minus1), scale1, w + 24);
                     weights8_in_order(v1.w, as_half2(minus1), scale1, w + 28);
-                    ok = mbar_wait(a_empty + 8 * a.s, a.phase ^ 1);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
+                    if (!__all_sync(0xffffffffu, a_free)) {
+                        ok = wait_all(a_empty + a_bar, a_phase);
+                        if (!ok) break;
+                    }
                     fence_after_sync();
                     tmem_st_32x32(a_mine + 64 * a.s, w);
+                    const bool read_now = __all_sync(0xffffffffu, q_there);
+                    if (read_now) read_codes();
                     tmem_st_wait();
                     fence_before_sync();
                     __syncwarp();
                     if (lane == 0) {
-                        if (PAIR) mbar_arrive_cluster_tmem(mapa_shared(a_full + 8 * a.s, 0));      // the leader's MMA thread waits for both CTAs
-                        else mbar_arrive(a_full + 8 * a.s);
+                        if (PAIR) mbar_arrive_cluster_tmem(mapa_shared(a_full + a_bar, 0));      // the leader's MMA thread waits for both CTAs
+                        else mbar_arrive(a_full + a_bar);
+                        if (read_now) mbar_arrive(q_empty + 8 * q.s);
                     }
+                    if (more && !read_now) {
+                        ok = wait_all(q_full + 8 * q.s, q.phase);
+                        if (!ok) break;
+                        read_codes();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(q_empty + 8 * q.s);
+                    }
+                    a.skip(step, t.stages);
                 }
-                if ((u & 3) == 3 || u == units - 1) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(s_empty + 8 * sc.s);
-                    sc.next(WT_SS);
-                }
-                q.next(t.q_stages);
-                a.next(t.a_stages);
-                if (++turn == WT_GROUPS) turn = 0;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s_empty + 8 * sc.s);
+                sc.next(WT_SS);
+            }
+            if (group >= (uint32_t)units) {      // a single unit: the second group has none
+                q.skip(units, t.q_stages);
+                a.skip(units, t.stages);
             }
         }
         if (!ok && lane == 0) atomicCAS(t.status, 0, 21);
@@ -225,24 +262,70 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
             fence_after_sync();
             const uint32_t tacc = tmem_base + acc.s * t.acc_stride + ((uint32_t)(quarter * 32) << 16);
             const int rows = min(t.bt, p.M - m0);
-            for (int c = 0; c < rows; c += 16) {
-                uint32_t r[16];
-                tmem_ld_32x16(tacc + c, r);
-                const int left = rows - c;
-                unsigned short res[16];
-                if (p.residual) {
-                    const __half* src = p.residual + (long long)(m0 + c) * p.ldr + n;
+            // A thread holds one column n of the result and consecutive rows m. Neighbouring threads swap halves so that the
+            // even one has (n, n + 1) of row m and the odd one of row m + 1: a store covers two rows of 64 bytes. The options
+            // are uniform and each is a loop of its own (as branches per element they took 84 cycles an element).
+            const int np = n & ~1, mp = m0 + (lane & 1);
+            const uint32_t mine = lane & 1 ? 0x3276u : 0x5410u;
+            auto load_residual = [&](int c, uint32_t* res) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) res[e] = in && e < left ? *reinterpret_cast<const unsigned short*>(src + e * p.ldr) : 0;
+                for (int i = 0; i < 8; ++i) {
+                    res[i] = 0;
+                    if (t.in_pairs) {
+                        if (in && c + 2 * i + (lane & 1) < rows) res[i] = *reinterpret_cast<const uint32_t*>(p.residual + (long long)(mp + c + 2 * i) * p.ldr + np);
+                    } else if (in) {
+                        const unsigned short* src = reinterpret_cast<const unsigned short*>(p.residual) + (long long)(m0 + c + 2 * i) * p.ldr + n;
+                        if (c + 2 * i < rows) res[i] = src[0];
+                        if (c + 2 * i + 1 < rows) res[i] |= (uint32_t)src[p.ldr] << 16;
+                    }
+                }
+            };
+            uint32_t next_res[8];
+            if (p.residual) load_residual(0, next_res);
+            for (int c = 0; c < rows; c += 16) {
+                uint32_t r[16], res[8];
+                tmem_ld_32x16(tacc + c, r);
+                if (p.residual) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) res[i] = next_res[i];
+                    if (c + 16 < rows) load_residual(c + 16, next_res);
                 }
                 tmem_ld_wait();
-                __half* dst = p.out + (long long)(m0 + c) * p.ldo + n;
+                float v[16];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    float v = fmaf(__uint_as_float(r[e]), OPERAND_UNSCALE, bias);
-                    if (p.act == KATZ_ACT_SILU) v = silu_f(v);
-                    if (p.residual) v += __half2float(__ushort_as_half(res[e]));
-                    if (in && e < left) dst[e * p.ldo] = __float2half_rn(v * p.out_scale);
+                for (int e = 0; e < 16; ++e) v[e] = fmaf(__uint_as_float(r[e]), OPERAND_UNSCALE, bias);
+                if (p.act == KATZ_ACT_SILU) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) v[e] = silu_f(v[e]);
+                }
+                if (p.residual) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if (t.in_pairs) res[i] = __byte_perm(res[i], __shfl_xor_sync(0xffffffffu, res[i], 1), mine);
+                        const float2 f = unpack_half2(res[i]);
+                        v[2 * i] += f.x;
+                        v[2 * i + 1] += f.y;
+                    }
+                }
+                uint32_t o[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i] = pack_half2(v[2 * i] * p.out_scale, v[2 * i + 1] * p.out_scale);
+                if (t.in_pairs) {
+                    __half* dst = p.out + (long long)(mp + c) * p.ldo + np;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        o[i] = __byte_perm(o[i], __shfl_xor_sync(0xffffffffu, o[i], 1), mine);
+                        if (in && c + 2 * i + (lane & 1) < rows) *reinterpret_cast<uint32_t*>(dst) = o[i];
+                        dst += 2 * p.ldo;
+                    }
+                } else if (in) {
+                    unsigned short* dst = reinterpret_cast<unsigned short*>(p.out) + (long long)(m0 + c) * p.ldo + n;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if (c + 2 * i < rows) dst[0] = (unsigned short)o[i];
+                        if (c + 2 * i + 1 < rows) dst[p.ldo] = (unsigned short)(o[i] >> 16);
+                        dst += 2 * p.ldo;
+                    }
                 }
             }
             fence_before_sync();
@@ -257,25 +340,31 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
     } else if (warp == WT_X) {
         // ---------------------------------------------------------------------------------------- x
         if (elect_one()) {
-            Ring x;
+            Ring a;
             uint32_t issued = 0;
             bool ok = true;
             for (int tile = item0; tile < total && ok; tile += item_stride) {
                 int m0, n0;
                 rows_of(tile, m0, n0);
-                for (int s = 0; s < steps; ++s) {
-                    if (!mbar_wait(x_empty + 8 * x.s, x.phase ^ 1)) { ok = false; break; }
-                    const uint32_t dst = smem_u32(smem + x.s * t.x_bytes);
+                for (int u = 0; u < units; ++u) {
+                    if (!mbar_wait(a_empty + 8 * a.s, a.phase ^ 1)) { ok = false; break; }
+                    const uint32_t dst = smem_u32(smem + a.s * t.x_bytes), half = t.x_bytes / 2;
+                    const bool two = u * 128 + 64 < p.K;      // a tile's last unit may be one box
                     if (PAIR) {
                         // both CTAs' bytes are counted on the leader's barrier, which the leader arms for both
-                        if (rank == 0) mbar_expect_tx(x_full + 8 * x.s, 2 * t.x_bytes);
-                        tma_load_2d_pair(dst, &tmX, s * 64, m0 + (int)rank * (t.bt / 2), mapa_shared(x_full + 8 * x.s, 0));
+                        const uint32_t bar = mapa_shared(a_full + 8 * a.s, 0);
+                        const int m = m0 + (int)rank * (t.bt / 2);
+                        if (rank == 0) mbar_expect_tx(a_full + 8 * a.s, two ? 2 * t.x_bytes : t.x_bytes);
+                        tma_load_2d_pair(dst, &tmX, u * 128, m, bar);
+                        if (two) tma_load_2d_pair(dst + half, &tmX, u * 128 + 64, m, bar);
                     } else {
-                        mbar_expect_tx(x_full + 8 * x.s, t.x_bytes);
-                        tma_load_2d(dst, &tmX, s * 64, m0, x_full + 8 * x.s);
+                        const uint32_t bar = a_full + 8 * a.s;
+                        mbar_expect_tx(bar, two ? t.x_bytes : half);
+                        tma_load_2d(dst, &tmX, u * 128, m0, bar);
+                        if (two) tma_load_2d(dst + half, &tmX, u * 128 + 64, m0, bar);
                     }
                     ++issued;
-                    x.next(t.x_stages);
+                    a.next(t.stages);
                 }
             }
             if (!ok) {
@@ -283,8 +372,8 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                 // copies in flight land before the CTA's shared memory is released (a pair's second CTA waits for the first
                 // in the cluster barrier of the teardown: its copies are counted on the leader's barriers)
                 if (rank == 0) {
-                    const uint32_t n = t.x_stages, first = issued > n ? issued - n : 0;
-                    for (uint32_t i = first; i < issued; ++i) mbar_wait(x_full + 8 * (i % n), (i / n) & 1);
+                    const uint32_t n = t.stages, first = issued > n ? issued - n : 0;
+                    for (uint32_t i = first; i < issued; ++i) mbar_wait(a_full + 8 * (i % n), (i / n) & 1);
                 }
             }
         }
@@ -292,31 +381,29 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
         // ---------------------------------------------------------------------------------------- MMA
         if (rank == 0 && elect_one()) {
             const uint32_t idesc = idesc_f16(PAIR ? 256 : 128, t.bt);
-            Ring x, a, acc;
+            Ring a, acc;
             bool ok = true;
             for (int tile = item0; tile < total && ok; tile += item_stride) {
                 if (!mbar_wait(acc_empty + 8 * acc.s, acc.phase ^ 1)) { ok = false; break; }
                 fence_after_sync();
                 const uint32_t tacc = tmem_base + acc.s * t.acc_stride;
-                for (int s = 0; s < steps; ++s) {
-                    if ((s & 1) == 0 && !mbar_wait(a_full + 8 * a.s, a.phase)) { ok = false; break; }
-                    if (!mbar_wait(x_full + 8 * x.s, x.phase)) { ok = false; break; }
+                for (int u = 0; u < units; ++u) {
+                    if (!mbar_wait(a_full + 8 * a.s, a.phase)) { ok = false; break; }
                     fence_after_sync();
-                    const uint64_t bd = smem_desc_sw128(smem_u32(smem + x.s * t.x_bytes));
-                    const uint32_t ta = a_base + 64 * a.s + 32 * (s & 1);
+                    const uint32_t xs = smem_u32(smem + a.s * t.x_bytes), ta = a_base + 64 * a.s;
+                    auto issue = [&](int b) {      // 64 k
+                        const uint64_t bd = smem_desc_sw128(xs + b * (t.x_bytes / 2));
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        if (PAIR) umma_f16_ta_pair(tacc, ta + 8 * k, bd + 2 * k, idesc, (s | k) != 0);
-                        else umma_f16_ta(tacc, ta + 8 * k, bd + 2 * k, idesc, (s | k) != 0);
-                    }
-                    if (PAIR) umma_commit_pair(x_empty + 8 * x.s, 3);
-                    else umma_commit(x_empty + 8 * x.s);
-                    x.next(t.x_stages);
-                    if ((s & 1) == 1 || s == steps - 1) {
-                        if (PAIR) umma_commit_pair(a_empty + 8 * a.s, 3);
-                        else umma_commit(a_empty + 8 * a.s);
-                        a.next(t.a_stages);
-                    }
+                        for (int k = 0; k < 4; ++k) {
+                            if (PAIR) umma_f16_ta_pair(tacc, ta + 32 * b + 8 * k, bd + 2 * k, idesc, (u | b | k) != 0);
+                            else umma_f16_ta(tacc, ta + 32 * b + 8 * k, bd + 2 * k, idesc, (u | b | k) != 0);
+                        }
+                    };
+                    issue(0);
+                    if (u * 128 + 64 < p.K) issue(1);
+                    if (PAIR) umma_commit_pair(a_empty + 8 * a.s, 3);
+                    else umma_commit(a_empty + 8 * a.s);
+                    a.next(t.stages);
                 }
                 if (ok) {
                     if (PAIR) umma_commit_pair(acc_full + 8 * acc.s, 3);
@@ -335,10 +422,10 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
             for (int tile = item0; tile < total && ok; tile += item_stride) {
                 int m0, n0;
                 rows_of(tile, m0, n0);
-                for (int s = 0; s < steps; s += 2) {
+                for (int u = 0; u < units; ++u) {
                     if (!mbar_wait(q_empty + 8 * q.s, q.phase ^ 1)) { ok = false; break; }
                     mbar_expect_tx(q_full + 8 * q.s, WT_Q_BYTES);
-                    tma_load_2d(smem_u32(q_ring + q.s * WT_Q_BYTES), &tmQ, s * 32, n0, q_full + 8 * q.s);
+                    tma_load_2d(smem_u32(q_ring + q.s * WT_Q_BYTES), &tmQ, u * 64, n0, q_full + 8 * q.s);
                     ++issued;
                     q.next(t.q_stages);
                 }
@@ -519,13 +606,15 @@ int linear_w4_tc05(const W4Params& p, cudaStream_t st) {
         for (int two = 0; two < 2; ++two) {
             if (two && p.N <= 128) continue;
             const int n_tiles = ceil_div(p.N, two ? 256 : 128), slots = two ? dev.pairs : dev.sms;
-            const int n_acc = bt <= 160 ? 2 : 1;      // three stages of 64 columns beside them
-            const long long waves = ceil_div_ll((long long)m_tiles * n_tiles, slots);
+            const long long tiles = (long long)m_tiles * n_tiles;
+            const int n_acc = bt <= 160 && tiles > slots ? 2 : 1;      // three stages of 64 columns beside them
+            const long long waves = ceil_div_ll(tiles, slots);
             double step = 2.0 * bt, load = (bt * (two ? 64.0 : 128.0) + 4096.0) / 48.0;
             if (load > step) step = load;
             if (step < 190.0) step = 190.0;
             const double drain = 600.0 + 8.0 * bt;
             const double cost = waves * (steps * step + (n_acc == 1 ? drain : 100.0)) + drain;
+            if (!two && bt > 192) continue;      // two stages of x would be all that fits
             if (cost < best) {
                 best = cost;
                 pair = two;
@@ -538,12 +627,14 @@ int linear_w4_tc05(const W4Params& p, cudaStream_t st) {
     }
     KATZ_CHECK_ARG((long long)t.m_tiles * t.n_tiles < (1ll << 30), KATZ_ESIZE);
     t.acc_stride = ceil_div(t.bt, 32) * 32;
-    t.x_bytes = t.bt * (pair ? 64 : 128);
-    t.q_stages = t.x_bytes <= 16384 ? WT_QS : 5;
+    t.x_bytes = t.bt * (pair ? 128 : 256);
+    t.q_stages = t.x_bytes <= 32768 ? WT_QS : 5;
     const int room = (WT_MAX_SMEM - WT_FIXED_SMEM - t.q_stages * WT_Q_BYTES) / t.x_bytes;
-    t.x_stages = room < WT_XS ? room : WT_XS;
     const int cols = (WT_TMEM_COLS - t.n_acc * t.acc_stride) / 64;
-    t.a_stages = cols < WT_AS ? cols : WT_AS;
+    t.stages = std::min(std::min(room, cols), WT_AS);
+    KATZ_CHECK_ARG(t.stages >= 3, KATZ_ESIZE);      // what a group skips at most between its units; holds for every tile above
+    t.in_pairs = ((p.N | p.ldo) & 1) == 0 && ((uintptr_t)p.out & 3) == 0 &&
+                 (!p.residual || ((p.ldr & 1) == 0 && ((uintptr_t)p.residual & 3) == 0));
     t.status = tc05_status_device_ptr();
     if (!t.status) return KATZ_ENOTREADY;
     CUtensorMap tx, tq;
@@ -552,7 +643,7 @@ int linear_w4_tc05(const W4Params& p, cudaStream_t st) {
     if (rc) return rc;
     rc = encode_rows(&tq, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_64B, p.q, p.K / 2, p.N, p.K / 2, 64, 128);
     if (rc) return rc;
-    const int smem = t.x_stages * t.x_bytes + t.q_stages * WT_Q_BYTES + WT_FIXED_SMEM;
+    const int smem = t.stages * t.x_bytes + t.q_stages * WT_Q_BYTES + WT_FIXED_SMEM;
     const int tiles = t.m_tiles * t.n_tiles;
     if (pair) launch_k_cluster(linear_w4_tc05_kernel<true>, 2 * (tiles < dev.pairs ? tiles : dev.pairs), WT_THREADS, smem, st, 2, tx, tq, p, t);
     else launch_k_cluster(linear_w4_tc05_kernel<false>, tiles < dev.sms ? tiles : dev.sms, WT_THREADS, smem, st, 1, tx, tq, p, t);
