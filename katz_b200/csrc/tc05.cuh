@@ -44,6 +44,27 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
     return false;
 }
 
+// The same for roles that wait long while other warps of the SM compute: the thread may be suspended for up to 20 us per
+// poll (it wakes when the phase completes) instead of polling at the expense of the others' issue slots. Bounded by time:
+// about two seconds.
+__device__ __forceinline__ bool mbar_wait_idle(uint32_t bar, uint32_t parity) {
+    const long long start = clock64();
+    do {
+        uint32_t ok;
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+            "selp.b32 %0, 1, 0, p;\n"
+            "}\n"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity), "r"(20000u)
+            : "memory");
+        if (ok) return true;
+    } while (clock64() - start < (1ll << 32));
+    return false;
+}
+
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"

@@ -4,16 +4,16 @@
 // The WEIGHT rows are the 128 rows of the MMA and the rows of x its columns (BT of them, any multiple of 16 up to 256), so a
 // few dozen rows of x waste nothing. The weights never exist in memory as fp16: warps unpack them in registers and write
 // them to TENSOR MEMORY, from where the MMA reads its A operand; shared memory carries the 4-bit codes and x only. One
-// persistent CTA per SM, sixteen warps:
-//   * warps 0-7 unpack: a warp owns 32 weight rows (its TMEM lane quarter, one row per thread) and 32 of a k-step's 64 k:
-//     16 bytes of codes from shared memory, 16 fp16 pairs to TMEM (tcgen05.st), a ring of 32-column stages;
-//   * warps 8-11: epilogue, one weight row per thread; for each row of x a warp stores 32 consecutive outputs (64 bytes);
-//   * warp 12: TMA loads of x (64 k per stage, 128-byte swizzle); warp 14: TMA loads of codes (128 k per stage, 64-byte
-//     swizzle), a ring of its own so that the HBM stream of codes runs ahead of what x's ring holds;
-//   * warp 15: scales and zero points of 512 k at a time, gathered into shared memory as fp16 (64 * scale);
-//   * warp 13: tcgen05.mma, D[128 x BT] += A[TMEM] B[x].
+// persistent CTA per SM, twenty warps:
+//   * warps 0-11 unpack, in three groups that take turns over units of 128 k: a warp owns 32 weight rows (its TMEM lane
+//     quarter, one row per thread), 64 bytes of codes from shared memory, 64 fp16 pairs to TMEM (tcgen05.st);
+//   * warps 12-15: epilogue, one weight row per thread; for each row of x a warp stores 32 consecutive outputs (64 bytes);
+//   * warp 16: TMA loads of x (128-byte swizzle) into the stages whose A the unpacking warps fill: one barrier says that both
+//     are there; warp 18: TMA loads of codes (64-byte swizzle), a ring of its own so that the HBM stream runs ahead;
+//   * warp 19: scales and zero points of 1024 k at a time, gathered into shared memory as fp16 (64 * scale);
+//   * warp 17: tcgen05.mma, D[128 x BT] += A[TMEM] B[x].
 // CTA pairs (PAIR): the MMA covers 256 weight rows, 128 from each CTA's tensor memory, and each CTA loads half of x's tile:
-// per k-step an SM then fetches BT * 64 + 4096 bytes instead of BT * 128 + 4096, where L2 was the bound.
+// per 64 k an SM then fetches BT * 64 + 4096 bytes instead of BT * 128 + 4096, where L2 was the bound.
 //
 // Every mbarrier wait is bounded (tc05.cuh): on a time-out the CTA records a status word, stops storing, frees its TMEM and
 // returns; the host reads the word with katz_tc05_status().
@@ -30,22 +30,26 @@ using namespace w4;
 
 int* tc05_status_device_ptr();   // defined next to the status word (gemm_tc05.cu)
 
-constexpr int WT_THREADS = 768;
-constexpr int WT_GROUPS = 2, WT_GROUP_WARPS = 8;               // unpacking warps
+constexpr int WT_THREADS = 640;
+constexpr int WT_GROUPS = 3, WT_GROUP_WARPS = 4;               // unpacking warps
 constexpr int WT_UNPACK_WARPS = WT_GROUPS * WT_GROUP_WARPS;
 constexpr int WT_EPILOGUE = WT_UNPACK_WARPS, WT_X = WT_EPILOGUE + 4, WT_MMA = WT_X + 1, WT_Q = WT_X + 2;   // first warp of each role
-constexpr int WT_AS = 6, WT_QS = 8, WT_SS = 3;                 // most stages of each ring
+constexpr int WT_AS = 6, WT_QS = 6, WT_SS = 2;                 // stages of each ring (WT_AS: at most)
+// A barrier's parity tells a group that the use before its own is over only if the group knows that the one before THAT is:
+// of A's stages it knows that unit n - WT_GROUPS - stages has been multiplied (its last wait), and must know it of n - 2
+// stages; of the codes' stages it knows the loads of its own units only, n - WT_GROUPS i, and must know that of n - WT_QS.
+static_assert(WT_QS % WT_GROUPS == 0, "the unit that used a stage of codes before must be one of the same group");
 constexpr int WT_Q_BYTES = 128 * 64;                           // 128 rows x 128 k of codes
-constexpr int WT_S_ROWS = 512 / 32;                            // groups of a scale block at most
+constexpr int WT_S_UNITS = 8, WT_S_ROWS = WT_S_UNITS * 128 / 32;      // a scale block: units of 128 k, groups at most
 constexpr int WT_SCALE_BYTES = WT_S_ROWS * 128 * 2, WT_ZERO_BYTES = WT_S_ROWS * 128;
 constexpr int WT_TMEM_COLS = 512;
 constexpr int WT_BARS = 2 * (WT_QS + WT_AS + WT_SS + 2);
-constexpr int WT_FIXED_SMEM = WT_SS * (WT_SCALE_BYTES + WT_ZERO_BYTES) + WT_BARS * 8 + 16 + 1024;
+constexpr int WT_FIXED_SMEM = WT_QS * WT_Q_BYTES + WT_SS * (WT_SCALE_BYTES + WT_ZERO_BYTES) + WT_BARS * 8 + 16 + 1024;
 constexpr int WT_MAX_SMEM = 232448;
 
 struct W4Tile {
     int bt, acc_stride, n_acc;                 // columns of a tile (rows of x), of an accumulator buffer; buffers
-    int stages, q_stages, x_bytes;              // x_bytes: of x in a stage of this CTA (two boxes of 64 k)
+    int stages, x_bytes;              // x_bytes: of x in a stage of this CTA (two boxes of 64 k)
     int m_tiles, n_tiles;                      // n_tiles: of 128 rows, of a pair's 256
     bool in_pairs;                             // out (and residual) allow 4-byte accesses to (n, n + 1), n even
     int* status;
@@ -88,7 +92,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char* q_ring = smem + t.stages * t.x_bytes;
-    unsigned char* s_ring = q_ring + t.q_stages * WT_Q_BYTES;
+    unsigned char* s_ring = q_ring + WT_QS * WT_Q_BYTES;
     unsigned char* z_ring = s_ring + WT_SS * WT_SCALE_BYTES;
     uint64_t* bars = reinterpret_cast<uint64_t*>(z_ring + WT_SS * WT_ZERO_BYTES);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + WT_BARS);
@@ -151,73 +155,76 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
 
     if (warp < WT_UNPACK_WARPS) {
         // ---------------------------------------------------------------------------------------- unpack
-        const int quarter = warp & 3, h = (warp >> 2) & 1;
-        const uint32_t group = warp / WT_GROUP_WARPS;
+        const int quarter = warp & 3, group = warp >> 2;
         const int row = quarter * 32 + lane;
-        const uint32_t a_mine = a_base + ((uint32_t)(quarter * 32) << 16) + 32 * h;
-        const uint32_t swz = (uint32_t)((row >> 1) & 3);
-        const uint32_t q_mine0 = row * 64 + (((uint32_t)(2 * h) ^ swz) << 4), q_mine1 = row * 64 + (((uint32_t)(2 * h + 1) ^ swz) << 4);
-        // The groups take turns over a tile's units. A warp has its next unit's codes in registers before it hands over the
-        // current one, and the two barriers it will need are polled once BEFORE the arithmetic, so that a barrier that has
-        // long been passed (the usual case) costs nothing: waiting where the data was needed, a unit took 1800 cycles for 330
-        // of arithmetic.
+        const uint32_t a_mine = a_base + ((uint32_t)(quarter * 32) << 16);
+        const uint32_t swz = (uint32_t)((row >> 1) & 3) << 4;
+        // The groups take turns over the CTA's units. A warp has its next unit's codes in registers before it hands over the
+        // current one, and polls the two barriers it will need once before the arithmetic, so that a barrier that has long
+        // been passed (the usual case) costs nothing. (Waiting where the data was needed, a warp took 1800 cycles for 330
+        // of arithmetic.)
         Ring q, a, sc;
-        q.skip(group, t.q_stages);
+        q.skip(group, WT_QS);
         a.skip(group, t.stages);
+        const int count = item0 < total ? ((total - 1 - item0) / item_stride + 1) * units : 0;
+        int now = 0, mine = group;      // this CTA's units so far; this warp's next one
         bool ok = true;
-        uint4 v0, v1;
-        auto read_codes = [&]() {
-            const unsigned char* codes = q_ring + q.s * WT_Q_BYTES;
-            v0 = *reinterpret_cast<const uint4*>(codes + q_mine0);
-            v1 = *reinterpret_cast<const uint4*>(codes + q_mine1);
-        };
+        uint4 v0, v1, v2, v3;
+        auto codes = [&](uint32_t c) { return *reinterpret_cast<const uint4*>(q_ring + q.s * WT_Q_BYTES + row * 64 + ((c << 4) ^ swz)); };
         auto wait_all = [&](uint32_t bar, uint32_t phase) { return __all_sync(0xffffffffu, mbar_wait(bar, phase)); };
-        if ((int)group < units && item0 < total) {
+        auto free_codes = [&]() {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_empty + 8 * q.s);
+        };
+        if (mine < count) {
             ok = wait_all(q_full + 8 * q.s, q.phase);
             if (ok) {
-                read_codes();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(q_empty + 8 * q.s);
+                v0 = codes(0), v1 = codes(1), v2 = codes(2), v3 = codes(3);
+                free_codes();
             }
         }
         for (int tile = item0; tile < total && ok; tile += item_stride) {
-            for (int u0 = 0; u0 < units && ok; u0 += 4) {
-                // both groups wait for every scale block, so that neither can be a whole ring ahead of the other
+            for (int u0 = 0; u0 < units && ok; u0 += WT_S_UNITS) {
+                // every group waits for every scale block, so that none can be a whole ring ahead of another
                 ok = wait_all(s_full + 8 * sc.s, sc.phase);
-                const int u1 = min(u0 + 4, units);
-                for (int u = u0 + (int)group; u < u1 && ok; u += 2) {
-                    const uint32_t step = u + 2 < units ? 2 : units - u + group;      // to this group's next unit
-                    const bool more = u + 2 < units || tile + item_stride < total;
-                    const uint32_t a_bar = 8 * a.s, a_phase = a.phase ^ 1;
-                    q.skip(step, t.q_stages);
+                const int u1 = min(u0 + WT_S_UNITS, units);
+                const int first = u0 + (mine - now);
+                for (int u = first; u < u1 && ok; u += WT_GROUPS) {
+                    const bool more = mine + WT_GROUPS < count;
+                    const uint32_t a_bar = 8 * a.s, a_phase = a.phase ^ 1, ta = a_mine + 64 * a.s;
+                    mine += WT_GROUPS;
+                    q.skip(WT_GROUPS, WT_QS);
+                    a.skip(WT_GROUPS, t.stages);
                     const bool a_free = mbar_try_wait(a_empty + a_bar, a_phase);
                     const bool q_there = more && mbar_try_wait(q_full + 8 * q.s, q.phase);
-                    const int k = (u & 3) * 128 + 64 * h, j0 = (k >> p.group_shift) * 128 + row, j1 = ((k + 32) >> p.group_shift) * 128 + row;
-                    const __half* scales = reinterpret_cast<const __half*>(s_ring + sc.s * WT_SCALE_BYTES);
-                    const __half2 scale0 = __half2half2(scales[j0]), scale1 = __half2half2(scales[j1]);
-                    uint32_t minus0 = 0xd480e408u, minus1 = minus0;      // (-(1024 + 8), -(64 + 8))
-                    if (p.zero) {
-                        const unsigned char* zeros = z_ring + sc.s * WT_ZERO_BYTES;
-                        minus0 = 0xd400e400u + 0x00100001u * zeros[j0];
-                        minus1 = 0xd400e400u + 0x00100001u * zeros[j1];
-                    }
+                    const __half* scales = reinterpret_cast<const __half*>(s_ring + sc.s * WT_SCALE_BYTES) + row;
+                    const unsigned char* zeros = z_ring + sc.s * WT_ZERO_BYTES + row;
+                    const int k = (u - u0) * 128;
                     uint32_t w[32];
-                    weights8_in_order(v0.x, as_half2(minus0), scale0, w);
-                    weights8_in_order(v0.y, as_half2(minus0), scale0, w + 4);
-                    weights8_in_order(v0.z, as_half2(minus0), scale0, w + 8);
-                    weights8_in_order(v0.w, as_half2(minus0), scale0, w + 12);
-                    weights8_in_order(v1.x, as_half2(minus1), scale1, w + 16);
-                    weights8_in_order(v1.y, as_half2(minus1), scale1, w + 20);
-                    weights8_in_order(v1.z, as_half2(minus1), scale1, w + 24);
-                    weights8_in_order(v1.w, as_half2(minus1), scale1, w + 28);
+                    auto unpack = [&](int k32, const uint4& v, uint32_t* o) {      // 32 k of one group
+                        const int j = ((k + 32 * k32) >> p.group_shift) * 128;
+                        const __half2 scale = __half2half2(scales[j]);
+                        uint32_t minus = 0xd480e408u;      // (-(1024 + 8), -(64 + 8))
+                        if (p.zero) minus = 0xd400e400u + 0x00100001u * zeros[j];
+                        weights8_in_order(v.x, as_half2(minus), scale, o);
+                        weights8_in_order(v.y, as_half2(minus), scale, o + 4);
+                        weights8_in_order(v.z, as_half2(minus), scale, o + 8);
+                        weights8_in_order(v.w, as_half2(minus), scale, o + 12);
+                    };
+                    unpack(0, v0, w);
+                    unpack(1, v1, w + 16);
                     if (!__all_sync(0xffffffffu, a_free)) {
                         ok = wait_all(a_empty + a_bar, a_phase);
                         if (!ok) break;
                     }
                     fence_after_sync();
-                    tmem_st_32x32(a_mine + 64 * a.s, w);
+                    tmem_st_32x32(ta, w);
                     const bool read_now = __all_sync(0xffffffffu, q_there);
-                    if (read_now) read_codes();
+                    if (read_now) v0 = codes(0), v1 = codes(1);
+                    unpack(2, v2, w);
+                    unpack(3, v3, w + 16);
+                    tmem_st_32x32(ta + 32, w);
+                    if (read_now) v2 = codes(2), v3 = codes(3);
                     tmem_st_wait();
                     fence_before_sync();
                     __syncwarp();
@@ -229,19 +236,14 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                     if (more && !read_now) {
                         ok = wait_all(q_full + 8 * q.s, q.phase);
                         if (!ok) break;
-                        read_codes();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(q_empty + 8 * q.s);
+                        v0 = codes(0), v1 = codes(1), v2 = codes(2), v3 = codes(3);
+                        free_codes();
                     }
-                    a.skip(step, t.stages);
                 }
+                now += u1 - u0;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(s_empty + 8 * sc.s);
                 sc.next(WT_SS);
-            }
-            if (group >= (uint32_t)units) {      // a single unit: the second group has none
-                q.skip(units, t.q_stages);
-                a.skip(units, t.stages);
             }
         }
         if (!ok && lane == 0) atomicCAS(t.status, 0, 21);
@@ -256,7 +258,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
             const int n = n0 + quarter * 32 + lane;
             const bool in = n < p.N;
             const float bias = p.bias && in ? __half2float(p.bias[n]) : 0.f;
-            ok = mbar_wait(acc_full + 8 * acc.s, acc.phase);
+            ok = mbar_wait_idle(acc_full + 8 * acc.s, acc.phase);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             fence_after_sync();
@@ -347,7 +349,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                 int m0, n0;
                 rows_of(tile, m0, n0);
                 for (int u = 0; u < units; ++u) {
-                    if (!mbar_wait(a_empty + 8 * a.s, a.phase ^ 1)) { ok = false; break; }
+                    if (!mbar_wait_idle(a_empty + 8 * a.s, a.phase ^ 1)) { ok = false; break; }
                     const uint32_t dst = smem_u32(smem + a.s * t.x_bytes), half = t.x_bytes / 2;
                     const bool two = u * 128 + 64 < p.K;      // a tile's last unit may be one box
                     if (PAIR) {
@@ -373,7 +375,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                 // in the cluster barrier of the teardown: its copies are counted on the leader's barriers)
                 if (rank == 0) {
                     const uint32_t n = t.stages, first = issued > n ? issued - n : 0;
-                    for (uint32_t i = first; i < issued; ++i) mbar_wait(a_full + 8 * (i % n), (i / n) & 1);
+                    for (uint32_t i = first; i < issued; ++i) mbar_wait_idle(a_full + 8 * (i % n), (i / n) & 1);
                 }
             }
         }
@@ -384,11 +386,11 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
             Ring a, acc;
             bool ok = true;
             for (int tile = item0; tile < total && ok; tile += item_stride) {
-                if (!mbar_wait(acc_empty + 8 * acc.s, acc.phase ^ 1)) { ok = false; break; }
+                if (!mbar_wait_idle(acc_empty + 8 * acc.s, acc.phase ^ 1)) { ok = false; break; }
                 fence_after_sync();
                 const uint32_t tacc = tmem_base + acc.s * t.acc_stride;
                 for (int u = 0; u < units; ++u) {
-                    if (!mbar_wait(a_full + 8 * a.s, a.phase)) { ok = false; break; }
+                    if (!mbar_wait_idle(a_full + 8 * a.s, a.phase)) { ok = false; break; }
                     fence_after_sync();
                     const uint32_t xs = smem_u32(smem + a.s * t.x_bytes), ta = a_base + 64 * a.s;
                     auto issue = [&](int b) {      // 64 k
@@ -423,30 +425,30 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                 int m0, n0;
                 rows_of(tile, m0, n0);
                 for (int u = 0; u < units; ++u) {
-                    if (!mbar_wait(q_empty + 8 * q.s, q.phase ^ 1)) { ok = false; break; }
+                    if (!mbar_wait_idle(q_empty + 8 * q.s, q.phase ^ 1)) { ok = false; break; }
                     mbar_expect_tx(q_full + 8 * q.s, WT_Q_BYTES);
                     tma_load_2d(smem_u32(q_ring + q.s * WT_Q_BYTES), &tmQ, u * 64, n0, q_full + 8 * q.s);
                     ++issued;
-                    q.next(t.q_stages);
+                    q.next(WT_QS);
                 }
             }
             if (!ok) {
                 atomicCAS(t.status, 0, 25);
-                const uint32_t n = t.q_stages, first = issued > n ? issued - n : 0;
-                for (uint32_t i = first; i < issued; ++i) mbar_wait(q_full + 8 * (i % n), (i / n) & 1);
+                const uint32_t n = WT_QS, first = issued > n ? issued - n : 0;
+                for (uint32_t i = first; i < issued; ++i) mbar_wait_idle(q_full + 8 * (i % n), (i / n) & 1);
             }
         }
     } else {
         // ---------------------------------------------------------------------------------------- scales, zero points
         Ring sc;
         bool ok = true;
-        const int per_block = 512 >> p.group_shift;
+        const int per_block = (WT_S_UNITS * 128) >> p.group_shift;
         const bool by_four = (p.J & 3) == 0 && ((uintptr_t)p.scale & 7) == 0;
         for (int tile = item0; tile < total && ok; tile += item_stride) {
             int m0, n0;
             rows_of(tile, m0, n0);
             for (int j0 = 0; j0 < p.J; j0 += per_block) {
-                ok = mbar_wait(s_empty + 8 * sc.s, sc.phase ^ 1);
+                ok = mbar_wait_idle(s_empty + 8 * sc.s, sc.phase ^ 1);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 __half* dst = reinterpret_cast<__half*>(s_ring + sc.s * WT_SCALE_BYTES);
@@ -628,11 +630,10 @@ int linear_w4_tc05(const W4Params& p, cudaStream_t st) {
     KATZ_CHECK_ARG((long long)t.m_tiles * t.n_tiles < (1ll << 30), KATZ_ESIZE);
     t.acc_stride = ceil_div(t.bt, 32) * 32;
     t.x_bytes = t.bt * (pair ? 128 : 256);
-    t.q_stages = t.x_bytes <= 32768 ? WT_QS : 5;
-    const int room = (WT_MAX_SMEM - WT_FIXED_SMEM - t.q_stages * WT_Q_BYTES) / t.x_bytes;
+    const int room = (WT_MAX_SMEM - WT_FIXED_SMEM) / t.x_bytes;
     const int cols = (WT_TMEM_COLS - t.n_acc * t.acc_stride) / 64;
     t.stages = std::min(std::min(room, cols), WT_AS);
-    KATZ_CHECK_ARG(t.stages >= 3, KATZ_ESIZE);      // what a group skips at most between its units; holds for every tile above
+    KATZ_CHECK_ARG(t.stages >= WT_GROUPS, KATZ_ESIZE);      // holds for every tile the choice above makes
     t.in_pairs = ((p.N | p.ldo) & 1) == 0 && ((uintptr_t)p.out & 3) == 0 &&
                  (!p.residual || ((p.ldr & 1) == 0 && ((uintptr_t)p.residual & 3) == 0));
     t.status = tc05_status_device_ptr();
@@ -643,7 +644,7 @@ int linear_w4_tc05(const W4Params& p, cudaStream_t st) {
     if (rc) return rc;
     rc = encode_rows(&tq, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_64B, p.q, p.K / 2, p.N, p.K / 2, 64, 128);
     if (rc) return rc;
-    const int smem = t.stages * t.x_bytes + t.q_stages * WT_Q_BYTES + WT_FIXED_SMEM;
+    const int smem = t.stages * t.x_bytes + WT_FIXED_SMEM;
     const int tiles = t.m_tiles * t.n_tiles;
     if (pair) launch_k_cluster(linear_w4_tc05_kernel<true>, 2 * (tiles < dev.pairs ? tiles : dev.pairs), WT_THREADS, smem, st, 2, tx, tq, p, t);
     else launch_k_cluster(linear_w4_tc05_kernel<false>, tiles < dev.sms ? tiles : dev.sms, WT_THREADS, smem, st, 1, tx, tq, p, t);
