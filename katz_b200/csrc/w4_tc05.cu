@@ -67,6 +67,26 @@ __device__ __forceinline__ void weights8_in_order(uint32_t w, __half2 minus, __h
     }
 }
 
+// Shared memory by 32-bit address: the aligned base of dynamic shared memory is an integer to the compiler, and through a
+// pointer made of it every access would be a generic one with 64-bit arithmetic.
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t a) {
+    unsigned short v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t lds8(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sts16(uint32_t a, __half v) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"(__half_as_ushort(v)) : "memory"); }
+__device__ __forceinline__ void sts8(uint32_t a, uint32_t v) { asm volatile("st.shared.u8 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
+
 // position in a ring of `n` stages
 struct Ring {
     uint32_t s = 0, phase = 0;
@@ -90,13 +110,10 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                                                                        const __grid_constant__ CUtensorMap tmQ, const W4Params p,
                                                                        const W4Tile t) {
     extern __shared__ unsigned char smem_raw[];
-    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    unsigned char* q_ring = smem + t.stages * t.x_bytes;
-    unsigned char* s_ring = q_ring + WT_QS * WT_Q_BYTES;
-    unsigned char* z_ring = s_ring + WT_SS * WT_SCALE_BYTES;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(z_ring + WT_SS * WT_ZERO_BYTES);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + WT_BARS);
-    const uint32_t q_full = smem_u32(bars), q_empty = q_full + 8 * WT_QS,
+    const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
+    const uint32_t q_ring = smem + t.stages * t.x_bytes, s_ring = q_ring + WT_QS * WT_Q_BYTES, z_ring = s_ring + WT_SS * WT_SCALE_BYTES,
+                   bars = z_ring + WT_SS * WT_ZERO_BYTES, tmem_slot = bars + WT_BARS * 8;
+    const uint32_t q_full = bars, q_empty = q_full + 8 * WT_QS,
                    a_full = q_empty + 8 * WT_QS, a_empty = a_full + 8 * WT_AS, s_full = a_empty + 8 * WT_AS,
                    s_empty = s_full + 8 * WT_SS, acc_full = s_empty + 8 * WT_SS, acc_empty = acc_full + 16;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -126,10 +143,10 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
     }
     if (warp == WT_MMA) {
         if (PAIR) {
-            tmem_alloc_pair(smem_u32(tmem_slot), WT_TMEM_COLS);
+            tmem_alloc_pair(tmem_slot, WT_TMEM_COLS);
             tmem_relinquish_pair();
         } else {
-            tmem_alloc(smem_u32(tmem_slot), WT_TMEM_COLS);
+            tmem_alloc(tmem_slot, WT_TMEM_COLS);
             tmem_relinquish();
         }
     }
@@ -137,7 +154,8 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
     __syncthreads();
     if (PAIR) cluster_sync_all();      // the peer's barriers are initialised before anything signals them
     fence_after_sync();
-    const uint32_t tmem_base = *tmem_slot;
+    uint32_t tmem_base;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot) : "memory");
     const uint32_t a_base = tmem_base + t.n_acc * t.acc_stride;
 
     const int units = (p.K + 127) >> 7;      // stages of 128 k
@@ -158,7 +176,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
         const int quarter = warp & 3, group = warp >> 2;
         const int row = quarter * 32 + lane;
         const uint32_t a_mine = a_base + ((uint32_t)(quarter * 32) << 16);
-        const uint32_t swz = (uint32_t)((row >> 1) & 3) << 4;
+        const uint32_t swz = (uint32_t)((row >> 1) & 3) << 4, q_mine = q_ring + row * 64;
         // The groups take turns over the CTA's units. A warp has its next unit's codes in registers before it hands over the
         // current one, and polls the two barriers it will need once before the arithmetic, so that a barrier that has long
         // been passed (the usual case) costs nothing. (Waiting where the data was needed, a warp took 1800 cycles for 330
@@ -170,7 +188,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
         int now = 0, mine = group;      // this CTA's units so far; this warp's next one
         bool ok = true;
         uint4 v0, v1, v2, v3;
-        auto codes = [&](uint32_t c) { return *reinterpret_cast<const uint4*>(q_ring + q.s * WT_Q_BYTES + row * 64 + ((c << 4) ^ swz)); };
+        auto codes = [&](uint32_t c) { return lds128(q_mine + q.s * WT_Q_BYTES + ((c << 4) ^ swz)); };
         auto wait_all = [&](uint32_t bar, uint32_t phase) { return __all_sync(0xffffffffu, mbar_wait(bar, phase)); };
         auto free_codes = [&]() {
             __syncwarp();
@@ -197,15 +215,14 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                     a.skip(WT_GROUPS, t.stages);
                     const bool a_free = mbar_try_wait(a_empty + a_bar, a_phase);
                     const bool q_there = more && mbar_try_wait(q_full + 8 * q.s, q.phase);
-                    const __half* scales = reinterpret_cast<const __half*>(s_ring + sc.s * WT_SCALE_BYTES) + row;
-                    const unsigned char* zeros = z_ring + sc.s * WT_ZERO_BYTES + row;
-                    const int k = (u - u0) * 128;
+                    const uint32_t scales = s_ring + sc.s * WT_SCALE_BYTES + row * 2, zeros = z_ring + sc.s * WT_ZERO_BYTES + row;
+                    const uint32_t k = (u - u0) * 128;
                     uint32_t w[32];
-                    auto unpack = [&](int k32, const uint4& v, uint32_t* o) {      // 32 k of one group
-                        const int j = ((k + 32 * k32) >> p.group_shift) * 128;
-                        const __half2 scale = __half2half2(scales[j]);
+                    auto unpack = [&](uint32_t k32, const uint4& v, uint32_t* o) {      // 32 k of one group
+                        const uint32_t j = ((k + 32 * k32) >> p.group_shift) * 128;
+                        const __half2 scale = as_half2(lds16(scales + 2 * j) * 0x10001u);
                         uint32_t minus = 0xd480e408u;      // (-(1024 + 8), -(64 + 8))
-                        if (p.zero) minus = 0xd400e400u + 0x00100001u * zeros[j];
+                        if (p.zero) minus = 0xd400e400u + 0x00100001u * lds8(zeros + j);
                         weights8_in_order(v.x, as_half2(minus), scale, o);
                         weights8_in_order(v.y, as_half2(minus), scale, o + 4);
                         weights8_in_order(v.z, as_half2(minus), scale, o + 8);
@@ -258,10 +275,6 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
             const int n = n0 + quarter * 32 + lane;
             const bool in = n < p.N;
             const float bias = p.bias && in ? __half2float(p.bias[n]) : 0.f;
-            ok = mbar_wait_idle(acc_full + 8 * acc.s, acc.phase);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            fence_after_sync();
             const uint32_t tacc = tmem_base + acc.s * t.acc_stride + ((uint32_t)(quarter * 32) << 16);
             const int rows = min(t.bt, p.M - m0);
             // A thread holds one column n of the result and consecutive rows m. Neighbouring threads swap halves so that the
@@ -282,15 +295,30 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                     }
                 }
             };
-            uint32_t next_res[8];
-            if (p.residual) load_residual(0, next_res);
+            if (p.residual) {      // into L2 while the main loop runs: a lane asks for a row's 64 bytes of this warp
+                const __half* line = p.residual + (long long)(m0 + lane) * p.ldr + n0 + quarter * 32;
+                if (n0 + quarter * 32 < p.N)
+                    for (int m = lane; m < rows; m += 32, line += 32 * p.ldr) asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
+            }
+            uint32_t next_res[2][8];      // the residual of the next two chunks
+            if (p.residual) {
+                load_residual(0, next_res[0]);
+                load_residual(16, next_res[1]);
+            }
+            ok = mbar_wait_idle(acc_full + 8 * acc.s, acc.phase);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            fence_after_sync();
             for (int c = 0; c < rows; c += 16) {
                 uint32_t r[16], res[8];
                 tmem_ld_32x16(tacc + c, r);
                 if (p.residual) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) res[i] = next_res[i];
-                    if (c + 16 < rows) load_residual(c + 16, next_res);
+                    for (int i = 0; i < 8; ++i) {
+                        res[i] = next_res[0][i];
+                        next_res[0][i] = next_res[1][i];
+                    }
+                    load_residual(c + 32, next_res[1]);      // nothing past the last row
                 }
                 tmem_ld_wait();
                 float v[16];
@@ -350,7 +378,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                 rows_of(tile, m0, n0);
                 for (int u = 0; u < units; ++u) {
                     if (!mbar_wait_idle(a_empty + 8 * a.s, a.phase ^ 1)) { ok = false; break; }
-                    const uint32_t dst = smem_u32(smem + a.s * t.x_bytes), half = t.x_bytes / 2;
+                    const uint32_t dst = smem + a.s * t.x_bytes, half = t.x_bytes / 2;
                     const bool two = u * 128 + 64 < p.K;      // a tile's last unit may be one box
                     if (PAIR) {
                         // both CTAs' bytes are counted on the leader's barrier, which the leader arms for both
@@ -392,7 +420,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                 for (int u = 0; u < units; ++u) {
                     if (!mbar_wait_idle(a_full + 8 * a.s, a.phase)) { ok = false; break; }
                     fence_after_sync();
-                    const uint32_t xs = smem_u32(smem + a.s * t.x_bytes), ta = a_base + 64 * a.s;
+                    const uint32_t xs = smem + a.s * t.x_bytes, ta = a_base + 64 * a.s;
                     auto issue = [&](int b) {      // 64 k
                         const uint64_t bd = smem_desc_sw128(xs + b * (t.x_bytes / 2));
 #pragma unroll
@@ -427,7 +455,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                 for (int u = 0; u < units; ++u) {
                     if (!mbar_wait_idle(q_empty + 8 * q.s, q.phase ^ 1)) { ok = false; break; }
                     mbar_expect_tx(q_full + 8 * q.s, WT_Q_BYTES);
-                    tma_load_2d(smem_u32(q_ring + q.s * WT_Q_BYTES), &tmQ, u * 64, n0, q_full + 8 * q.s);
+                    tma_load_2d(q_ring + q.s * WT_Q_BYTES, &tmQ, u * 64, n0, q_full + 8 * q.s);
                     ++issued;
                     q.next(WT_QS);
                 }
@@ -451,8 +479,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                 ok = mbar_wait_idle(s_empty + 8 * sc.s, sc.phase ^ 1);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                __half* dst = reinterpret_cast<__half*>(s_ring + sc.s * WT_SCALE_BYTES);
-                unsigned char* zdst = z_ring + sc.s * WT_ZERO_BYTES;
+                const uint32_t dst = s_ring + sc.s * WT_SCALE_BYTES + 2 * lane, zdst = z_ring + sc.s * WT_ZERO_BYTES + lane;
                 // groups past the last and rows past the last get zeros: their weights are zeros
                 // (every load of a batch is requested before the first is used: one round trip a batch, not one a load)
                 if (by_four) {
@@ -468,11 +495,11 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                         for (int u = 0; u < 8; ++u) {
                             const int i = b + u;
                             if (i >= per_block) break;
-                            __half* d = dst + (i & ~3) * 128 + lane + 32 * (i & 3);
-                            d[0] = __float2half_rn(__uint_as_float(v[u].x << 16) * OPERAND_SCALE);
-                            d[128] = __float2half_rn(__uint_as_float(v[u].x & 0xffff0000u) * OPERAND_SCALE);
-                            d[256] = __float2half_rn(__uint_as_float(v[u].y << 16) * OPERAND_SCALE);
-                            d[384] = __float2half_rn(__uint_as_float(v[u].y & 0xffff0000u) * OPERAND_SCALE);
+                            const uint32_t d = dst + 2 * ((i & ~3) * 128 + 32 * (i & 3));
+                            sts16(d, __float2half_rn(__uint_as_float(v[u].x << 16) * OPERAND_SCALE));
+                            sts16(d + 256, __float2half_rn(__uint_as_float(v[u].x & 0xffff0000u) * OPERAND_SCALE));
+                            sts16(d + 512, __float2half_rn(__uint_as_float(v[u].y << 16) * OPERAND_SCALE));
+                            sts16(d + 768, __float2half_rn(__uint_as_float(v[u].y & 0xffff0000u) * OPERAND_SCALE));
                         }
                     }
                 } else {
@@ -486,7 +513,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
 #pragma unroll
                         for (int u = 0; u < 16; ++u) {
                             const int i = b + u;
-                            dst[(i >> 2) * 128 + lane + 32 * (i & 3)] = __float2half_rn(bf16_bits_to_float(v[u]) * OPERAND_SCALE);
+                            sts16(dst + 2 * ((i >> 2) * 128 + 32 * (i & 3)), __float2half_rn(bf16_bits_to_float(v[u]) * OPERAND_SCALE));
                         }
                     }
                 }
@@ -501,7 +528,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
 #pragma unroll
                         for (int u = 0; u < 16; ++u) {
                             const int i = b + u;
-                            zdst[(i >> 2) * 128 + lane + 32 * (i & 3)] = v[u];
+                            sts8(zdst + (i >> 2) * 128 + 32 * (i & 3), v[u]);
                         }
                     }
                 }
