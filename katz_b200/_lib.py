@@ -131,7 +131,7 @@ SIGNATURES = {
     "katz_quantize_w4_f16": (_I, [_V, _L, _V, _V, _I, _I, _I, _V]),
     "katz_dequantize_w4_f16": (_I, [_V, _V, _V, _V, _L, _I, _I, _I, _V]),
     "katz_linear_w4_f16": (_I, [_V, _L, _V, _V, _V, _I, _V, _L, _I, _I, _I, _V, _V, _L, _I, _F, _V]),
-    "katz_residual_norm_f16": (_I, [POINTER(ResidualNormArgs), _V]),
+    "katz_residual_norm_f16": (_I, [_V, _V]),      # a ResidualNormArgs, or its bytes
 }
 
 _lib = None

@@ -2,6 +2,7 @@
 torch stream. No op here computes anything in torch; a missing library or a failing launch raises KatzError."""
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -180,46 +181,66 @@ def linear(x, w, bias=None, residual=None, act=ACT_NONE, rowvec=None, rows_per_b
     return out
 
 
-def _same_device(t, device, name):
-    if t.device != device:
-        raise KatzError("%s is on %s, not on %s" % (name, t.device, device))
-    return t
+_F16, _F32, _BF16, _U8 = torch.float16, torch.float32, torch.bfloat16, torch.uint8
+# the raw handle of a device's current stream; torch.cuda.current_stream() builds an object around it, which takes 3 us, a
+# quarter of a small call
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _call_on(device, name, *args):
-    """Launch on the current stream of `device`, which need not be the current device."""
-    if device.index == torch.cuda.current_device():
-        call(name, *args, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+def _call_on(index, name, *args):
+    """Launch on the current stream of CUDA device `index`, which need not be the current device."""
+    if index == torch.cuda.current_device():
+        call(name, *args, _raw_stream(index))
         return
-    with torch.cuda.device(device):
-        call(name, *args, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+    with torch.cuda.device(index):
+        call(name, *args, _raw_stream(index))
 
 
-def _rows_ok(t, M, N):
-    """[M, N] with unit column stride and rows that do not overlap."""
-    return t.dim() == 2 and t.shape == (M, N) and (t.stride(1) == 1 or N == 1) and (M < 2 or t.stride(0) >= N)
+def _expect(t, what, name, dtype, index):
+    """t is a tensor of `dtype` on CUDA device `index` (None: on any)."""
+    at = t.get_device()
+    if t.dtype is not dtype or at < 0 or (index is not None and at != index):
+        where = "" if index is None else " %d" % index
+        raise KatzError("%s: %s must be a %s tensor on CUDA device%s (got %s on %s)" % (what, name, dtype, where, t.dtype, t.device))
+    return at
+
+
+def _row_stride(t, what, name, M, N):
+    """Row stride of an [M, N] tensor with unit column stride and rows that do not overlap."""
+    if t.shape != (M, N):
+        raise KatzError("%s: %s must be %s (got %s)" % (what, name, (M, N), tuple(t.shape)))
+    ld, one = t.stride()
+    if one != 1 and N != 1:
+        raise KatzError("%s: %s must have unit column stride (got strides %s)" % (what, name, t.stride()))
+    if M < 2:
+        return N
+    if ld < N:
+        raise KatzError("%s: the rows of %s overlap (strides %s)" % (what, name, t.stride()))
+    return ld
 
 
 def _w4_check(what, q, scale, zero, group):
-    """(N, K) of a 4-bit weight; see quantize_w4 for the format."""
+    """(device index, N, K) of a 4-bit weight; see quantize_w4 for the format."""
     if group not in (32, 64, 128):
         raise KatzError("%s: group must be 32, 64 or 128 (got %r)" % (what, group))
-    if q.dtype != torch.uint8 or not q.is_cuda or q.dim() != 2 or not q.is_contiguous():
-        raise KatzError("%s: q must be a contiguous CUDA uint8 [N, K/2] tensor" % what)
-    N, K = q.shape[0], 2 * q.shape[1]
+    index = _expect(q, what, "q", _U8, None)
+    if q.dim() != 2 or not q.is_contiguous():
+        raise KatzError("%s: q must be a contiguous [N, K/2] tensor" % what)
+    N, K = q.shape
+    K *= 2
     if K == 0 or K % 32:
         raise KatzError("%s: K must be a positive multiple of 32 (got %d)" % (what, K))
     if q.data_ptr() % 16:
         raise KatzError("%s: q must start on a 16-byte boundary" % what)
     shape = (N, (K + group - 1) // group)
-    if scale.dtype != torch.bfloat16 or scale.shape != shape or not scale.is_contiguous():
-        raise KatzError("%s: scale must be a contiguous bf16 [N, ceil(K/group)] = %s tensor" % (what, shape))
-    _same_device(scale, q.device, "scale")
+    _expect(scale, what, "scale", _BF16, index)
+    if scale.shape != shape or not scale.is_contiguous():
+        raise KatzError("%s: scale must be a contiguous [N, ceil(K/group)] = %s tensor" % (what, shape))
     if zero is not None:
-        if zero.dtype != torch.uint8 or zero.shape != shape or not zero.is_contiguous():
-            raise KatzError("%s: zero must be a contiguous uint8 %s tensor" % (what, shape))
-        _same_device(zero, q.device, "zero")
-    return N, K
+        _expect(zero, what, "zero", _U8, index)
+        if zero.shape != shape or not zero.is_contiguous():
+            raise KatzError("%s: zero must be a contiguous %s tensor" % (what, shape))
+    return index, N, K
 
 
 def quantize_w4(w, group=64, out=None):
@@ -228,37 +249,40 @@ def quantize_w4(w, group=64, out=None):
     64 or 128) consecutive k of a row, the last group may be short; weight = scale * (code - 8), |code - 8| <= 7, ties to even.
     A group that holds an infinity or a NaN reads back as NaN. Rows are independent: row slices of (q, scale) are the 4-bit
     form of the same rows of w. `out` = (q, scale) rewrites an existing pair, as after an adapter switch."""
-    _f16(w, "w")
+    index = _expect(w, "quantize_w4", "w", _F16, None)
     if w.dim() != 2 or w.shape[1] == 0 or w.shape[1] % 32:
         raise KatzError("quantize_w4: w must be [N, K] with K a positive multiple of 32 (got %s)" % (tuple(w.shape),))
     N, K = w.shape
-    if not _rows_ok(w, N, K) or not _al16(w) or (N > 1 and w.stride(0) % 8):
-        raise KatzError("quantize_w4: w must have unit column stride and 16-byte aligned rows")
+    ld = _row_stride(w, "quantize_w4", "w", N, K)
+    if w.data_ptr() % 16 or ld % 8:
+        raise KatzError("quantize_w4: the rows of w must start on 16-byte boundaries")
     if group not in (32, 64, 128):
         raise KatzError("quantize_w4: group must be 32, 64 or 128 (got %r)" % (group,))
     if out is None:
-        out = (torch.empty((N, K // 2), dtype=torch.uint8, device=w.device),
-               torch.empty((N, (K + group - 1) // group), dtype=torch.bfloat16, device=w.device))
-    q, scale = out
-    if _w4_check("quantize_w4", q, scale, None, group) != (N, K):
-        raise KatzError("quantize_w4: out does not match w %s" % (tuple(w.shape),))
-    _same_device(q, w.device, "out")
+        q, scale = w.new_empty((N, K // 2), dtype=_U8), w.new_empty((N, (K + group - 1) // group), dtype=_BF16)
+    else:
+        q, scale = out
+        if _w4_check("quantize_w4", q, scale, None, group) != (index, N, K):
+            raise KatzError("quantize_w4: out does not match w %s on %s" % (tuple(w.shape), w.device))
     if N:
-        _call_on(w.device, "katz_quantize_w4_f16", w.data_ptr(), max(w.stride(0), K), q.data_ptr(), scale.data_ptr(), N, K, group)
+        _call_on(index, "katz_quantize_w4_f16", w.data_ptr(), ld, q.data_ptr(), scale.data_ptr(), N, K, group)
     return q, scale
 
 
 def dequantize_w4(q, scale, zero=None, group=64, out=None):
     """4-bit weights -> fp16 [N, K] = scale * (code - zero), rounded once. `zero`: uint8 of scale's shape, 0..15 (None: 8)."""
-    N, K = _w4_check("dequantize_w4", q, scale, zero, group)
+    index, N, K = _w4_check("dequantize_w4", q, scale, zero, group)
+    ld = K
     if out is None:
-        out = torch.empty((N, K), dtype=torch.float16, device=q.device)
-    _same_device(_f16(out, "out"), q.device, "out")
-    if not _rows_ok(out, N, K) or not _al16(out) or (N > 1 and out.stride(0) % 8):
-        raise KatzError("dequantize_w4: out must be [N, K] with unit column stride and 16-byte aligned rows")
+        out = q.new_empty((N, K), dtype=_F16)
+    else:
+        _expect(out, "dequantize_w4", "out", _F16, index)
+        ld = _row_stride(out, "dequantize_w4", "out", N, K)
+        if out.data_ptr() % 16 or ld % 8:
+            raise KatzError("dequantize_w4: the rows of out must start on 16-byte boundaries")
     if N:
-        _call_on(q.device, "katz_dequantize_w4_f16", q.data_ptr(), scale.data_ptr(), zero.data_ptr() if zero is not None else None,
-                 out.data_ptr(), max(out.stride(0), K), N, K, group)
+        _call_on(index, "katz_dequantize_w4_f16", q.data_ptr(), scale.data_ptr(), zero.data_ptr() if zero is not None else None,
+                 out.data_ptr(), ld, N, K, group)
     return out
 
 
@@ -267,34 +291,36 @@ def linear_w4(x, q, scale, zero=None, group=64, bias=None, residual=None, act=AC
     (+bias) -> act -> (+residual) * out_scale, fp32 accumulation, one rounding. Any M (0 included) and N.
     `x`, `residual`, `out` may be row-strided 2-D views (unit column stride); `out` may be `residual`. Scales of 2^-23 to 64
     are covered: the weights of larger ones overflow fp16 to infinity, those of smaller ones lose bits."""
-    _f16(x, "x")
-    N, K = _w4_check("linear_w4", q, scale, zero, group)
-    dev = x.device
-    _same_device(q, dev, "q")
-    M = x.shape[0]
-    if not _rows_ok(x, M, K):
-        raise KatzError("linear_w4: x must be [M, %d] with unit column stride (got %s, strides %s)" % (K, tuple(x.shape), x.stride()))
-    if act not in (ACT_NONE, ACT_SILU):
+    index, N, K = _w4_check("linear_w4", q, scale, zero, group)
+    _expect(x, "linear_w4", "x", _F16, index)
+    M = x.shape[0] if x.dim() == 2 else -1
+    ldx = _row_stride(x, "linear_w4", "x", M, K)
+    if act != ACT_NONE and act != ACT_SILU:
         raise KatzError("linear_w4: unknown activation %r" % (act,))
+    ldo = N
     if out is None:
-        out = torch.empty((M, N), dtype=torch.float16, device=dev)
+        out = x.new_empty((M, N))
     else:
-        _same_device(_f16(out, "out"), dev, "out")
-        if not _rows_ok(out, M, N) or (M and N and out.data_ptr() == x.data_ptr()):
-            raise KatzError("linear_w4: bad out")
+        _expect(out, "linear_w4", "out", _F16, index)
+        ldo = _row_stride(out, "linear_w4", "out", M, N)
+        if M and N and out.data_ptr() == x.data_ptr():
+            raise KatzError("linear_w4: out must not be x")
+    bias_p = residual_p = None
+    ldr = 0
     if bias is not None:
-        _same_device(_f16(bias, "bias"), dev, "bias")
+        _expect(bias, "linear_w4", "bias", _F16, index)
         if bias.shape != (N,) or not bias.is_contiguous():
             raise KatzError("linear_w4: bias must be a contiguous [N] tensor")
+        bias_p = bias.data_ptr()
     if residual is not None:
-        _same_device(_f16(residual, "residual"), dev, "residual")
-        if not _rows_ok(residual, M, N) or (residual.data_ptr() == out.data_ptr() and M > 1 and residual.stride(0) != out.stride(0)):
-            raise KatzError("linear_w4: bad residual")
+        _expect(residual, "linear_w4", "residual", _F16, index)
+        ldr = _row_stride(residual, "linear_w4", "residual", M, N)
+        residual_p = residual.data_ptr()
+        if ldr != ldo and residual_p == out.data_ptr():
+            raise KatzError("linear_w4: residual starts where out does, with another row stride")
     if M and N:
-        _call_on(dev, "katz_linear_w4_f16", x.data_ptr(), max(x.stride(0), K), q.data_ptr(), scale.data_ptr(),
-                 zero.data_ptr() if zero is not None else None, group, out.data_ptr(), max(out.stride(0), N), M, N, K,
-                 bias.data_ptr() if bias is not None else None, residual.data_ptr() if residual is not None else None,
-                 max(residual.stride(0), N) if residual is not None else 0, act, float(out_scale))
+        _call_on(index, "katz_linear_w4_f16", x.data_ptr(), ldx, q.data_ptr(), scale.data_ptr(), zero.data_ptr() if zero is not None else None,
+                 group, out.data_ptr(), ldo, M, N, K, bias_p, residual_p, ldr, act, out_scale)
     return out
 
 
@@ -452,36 +478,61 @@ class Norm:
         self.code = _lib.NORM_LAYER if kind == "layer" else _lib.NORM_RMS
 
 
+_RESIDUAL_NORM_ARGS = struct.Struct("=11Q14q6i3f4x")      # katz_residual_norm_args
+
+
 def _row_strides(t, name, shape):
     """(batch, token) strides of an activation [rows, C] or [B, S, C] of the given shape with unit channel stride."""
-    if t.shape != shape or (t.stride(-1) != 1 and shape[-1] != 1):
-        raise KatzError("residual_norm: %s must be %s with unit channel stride (got %s, strides %s)" % (name, tuple(shape), tuple(t.shape), t.stride()))
-    return (t.stride(0) if len(shape) == 3 and shape[0] > 1 else 0), (t.stride(-2) if shape[-2] > 1 else 0)
+    st = t.stride()
+    if t.shape != shape or (st[-1] != 1 and shape[-1] != 1):
+        raise KatzError("residual_norm: %s must be %s with unit channel stride (got %s, strides %s)" % (name, tuple(shape), tuple(t.shape), st))
+    if len(st) == 2:
+        return 0, (st[0] if shape[0] > 1 else 0)
+    return (st[0] if shape[0] > 1 else 0), (st[1] if shape[1] > 1 else 0)
 
 
-def _written_rows(t, name, shape, dtype, device):
-    if t.dtype != dtype or t.device != device:
-        raise KatzError("residual_norm: %s must be a %s tensor on %s" % (name, dtype, device))
+def _written_rows(t, name, shape, B, S, C):
     sb, ss = _row_strides(t, name, shape)
-    C, S = shape[-1], shape[-2]
-    if (S > 1 and ss < C) or (len(shape) == 3 and shape[0] > 1 and sb < (S - 1) * ss + C):
-        raise KatzError("residual_norm: the rows of %s overlap" % name)
+    if (S > 1 and ss < C) or (B > 1 and sb < (S - 1) * ss + C):
+        raise KatzError("residual_norm: the rows of %s overlap (strides %s)" % (name, t.stride()))
     return sb, ss
 
 
-def _vector_strides(t, name, shape, device):
-    """(batch, token) strides of a gate, scale or shift: [C], [B, C] ([rows, C] for a 2-D x) or [B, S, C], sizes of 1 broadcast."""
-    _same_device(_f16(t, name), device, name)
-    d, C = t.dim(), shape[-1]
-    if d == 0 or d > len(shape) or t.shape[-1] != C or (t.stride(-1) != 1 and C != 1):
-        raise KatzError("residual_norm: %s %s does not fit x %s (unit channel stride)" % (name, tuple(t.shape), tuple(shape)))
+def _vector(t, name, shape, index):
+    """(address, batch stride, token stride) of a gate, scale or shift: [C], [B, C] ([rows, C] for a 2-D x) or [B, S, C], sizes
+    of 1 broadcast."""
+    if t is None:
+        return 0, 0, 0
+    _expect(t, "residual_norm", name, _F16, index)
+    ts, st = t.shape, t.stride()
+    d = len(ts)
+    ok = 0 < d <= len(shape) and ts[-1] == shape[-1] and (st[-1] == 1 or ts[-1] == 1)
+    strides = [0, 0]
+    first = 1 if len(shape) == 2 else 0      # a 2-D x is one batch of rows
     for i in range(d - 1):
-        if t.shape[i] != shape[i] and t.shape[i] != 1:
-            raise KatzError("residual_norm: %s %s does not fit x %s" % (name, tuple(t.shape), tuple(shape)))
-    st = [t.stride(i) if t.shape[i] != 1 else 0 for i in range(d - 1)]
-    if len(shape) == 2:
-        return 0, st[0] if st else 0
-    return (st + [0, 0])[:2]
+        if ts[i] == 1:
+            continue
+        ok = ok and ts[i] == shape[i]
+        if not ok:
+            break
+        strides[first + i] = st[i]
+    if not ok:
+        raise KatzError("residual_norm: %s %s (strides %s) does not fit x %s" % (name, tuple(ts), st, tuple(shape)))
+    return t.data_ptr(), strides[0], strides[1]
+
+
+def _norm_vectors(norm, side, C, index):
+    """(kind, eps, address of weight, address of bias)"""
+    if norm is None:
+        return _lib.NORM_NONE, 0.0, 0, 0
+    at = []
+    for v in (norm.weight, norm.bias):
+        if v is not None:
+            _expect(v, "residual_norm", side, _F16, index)
+            if v.shape != (C,) or not v.is_contiguous():
+                raise KatzError("residual_norm: weight and bias of %s must be contiguous [C] tensors" % side)
+        at.append(v.data_ptr() if v is not None else 0)
+    return norm.code, norm.eps, at[0], at[1]
 
 
 def residual_norm(x, y=None, gate=None, post=None, pre=None, scale=None, shift=None, residual_scale=1.0, out=None, normed=None):
@@ -492,10 +543,18 @@ def residual_norm(x, y=None, gate=None, post=None, pre=None, scale=None, shift=N
     or [rows, C]); sizes of 1 broadcast and any may be a view into a wider row. h has x's type, z is fp16 and None without
     `pre`; both are rounded once, z from the unrounded h. Without y, h is residual_scale * x (x itself where that is 1 and no
     `out` is given). `out` (for h) may be x, `normed` (for z) may be y; all last strides are 1."""
-    if not x.is_cuda or x.dtype not in (torch.float16, torch.float32):
-        raise KatzError("x must be a CUDA fp16 or fp32 tensor (got %s on %s)" % (x.dtype, x.device))
-    shape, dev = x.shape, x.device
-    if len(shape) not in (2, 3) or not 0 < shape[-1] <= _lib.RESIDUAL_NORM_MAX_C:
+    dtype = x.dtype
+    if dtype is not _F16 and dtype is not _F32:
+        raise KatzError("residual_norm: x must be a CUDA fp16 or fp32 tensor (got %s on %s)" % (dtype, x.device))
+    index = _expect(x, "residual_norm", "x", dtype, None)
+    shape = x.shape
+    if len(shape) == 3:
+        B, S, C = shape
+    elif len(shape) == 2:
+        B, (S, C) = 1, shape
+    else:
+        B = S = C = 0
+    if not 0 < C <= _lib.RESIDUAL_NORM_MAX_C:
         raise KatzError("residual_norm: x must be [rows, C] or [B, S, C] with 1 <= C <= %d (got %s)" % (_lib.RESIDUAL_NORM_MAX_C, tuple(shape)))
     if y is None and (gate is not None or post is not None):
         raise KatzError("residual_norm: gate and post need y")
@@ -503,54 +562,45 @@ def residual_norm(x, y=None, gate=None, post=None, pre=None, scale=None, shift=N
         raise KatzError("residual_norm: scale, shift and normed need pre")
     if y is None and pre is None:
         raise KatzError("residual_norm: neither y nor pre: nothing to compute")
-    a = _lib.ResidualNormArgs()
-    a.x = x.data_ptr()
-    a.x_sb, a.x_ss = _row_strides(x, "x", shape)
-    a.B, a.S, a.C = (shape[0] if len(shape) == 3 else 1), shape[-2], shape[-1]
-    a.x_dtype = _lib.KATZ_DTYPE_F16 if x.dtype == torch.float16 else _lib.KATZ_DTYPE_F32
-    a.residual_scale = residual_scale
+    x_p = x.data_ptr()
+    x_sb, x_ss = _row_strides(x, "x", shape)
+    y_p = y_sb = y_ss = 0
     if y is not None:
-        _same_device(_f16(y, "y"), dev, "y")
-        a.y = y.data_ptr()
-        a.y_sb, a.y_ss = _row_strides(y, "y", shape)
-    if gate is not None:
-        a.gate = gate.data_ptr()
-        a.gate_sb, a.gate_ss = _vector_strides(gate, "gate", shape, dev)
-    if scale is not None:
-        a.scale = scale.data_ptr()
-        a.scale_sb, a.scale_ss = _vector_strides(scale, "scale", shape, dev)
-    if shift is not None:
-        a.shift = shift.data_ptr()
-        a.shift_sb, a.shift_ss = _vector_strides(shift, "shift", shape, dev)
-    for side, norm in (("post", post), ("pre", pre)):
-        if norm is None:
-            continue
-        for part in ("weight", "bias"):
-            v = getattr(norm, part)
-            if v is not None:
-                _same_device(_f16(v, "%s.%s" % (side, part)), dev, "%s.%s" % (side, part))
-                if v.shape != (shape[-1],) or not v.is_contiguous():
-                    raise KatzError("residual_norm: %s.%s must be a contiguous [C] tensor" % (side, part))
-                setattr(a, "%s_%s" % (side, part), v.data_ptr())
-    if post is not None:
-        a.post_kind, a.post_eps = post.code, post.eps
-    h, z = out, None
-    if out is None:
-        h = x if y is None and residual_scale == 1.0 else torch.empty(shape, dtype=x.dtype, device=dev)
-    if h is not x or out is not None:
-        a.h = h.data_ptr()
-        a.h_sb, a.h_ss = _written_rows(h, "out", shape, x.dtype, dev)
-    if pre is not None:
-        a.pre_kind, a.pre_eps = pre.code, pre.eps
-        z = torch.empty(shape, dtype=torch.float16, device=dev) if normed is None else normed
-        a.z = z.data_ptr()
-        a.z_sb, a.z_ss = _written_rows(z, "normed", shape, torch.float16, dev)
-    if x.numel() == 0:
-        return h, z
-    if (a.h and (a.h == a.y or a.h == a.z or (a.h == a.x and (a.h_sb, a.h_ss) != (a.x_sb, a.x_ss)))) \
-            or (a.z and (a.z == a.x or (a.z == a.y and (a.z_sb, a.z_ss) != (a.y_sb, a.y_ss)))):
-        raise KatzError("residual_norm: out may only be x, normed may only be y, with the same strides")
-    _call_on(dev, "katz_residual_norm_f16", ctypes.byref(a))
+        _expect(y, "residual_norm", "y", _F16, index)
+        y_sb, y_ss = _row_strides(y, "y", shape)
+        y_p = y.data_ptr()
+    gate_p, gate_sb, gate_ss = _vector(gate, "gate", shape, index)
+    scale_p, scale_sb, scale_ss = _vector(scale, "scale", shape, index)
+    shift_p, shift_sb, shift_ss = _vector(shift, "shift", shape, index)
+    post_kind, post_eps, post_w, post_b = _norm_vectors(post, "post", C, index)
+    pre_kind, pre_eps, pre_w, pre_b = _norm_vectors(pre, "pre", C, index)
+    h, h_p, h_sb, h_ss = out, 0, S * C, C
+    if out is not None:
+        _expect(out, "residual_norm", "out", dtype, index)
+        h_sb, h_ss = _written_rows(out, "out", shape, B, S, C)
+        h_p = out.data_ptr()
+        if h_p == y_p or (h_p == x_p and (h_sb, h_ss) != (x_sb, x_ss)):
+            raise KatzError("residual_norm: out may be x (with the same strides), not y")
+    elif y is None and residual_scale == 1.0:
+        h = x
+    else:
+        h = x.new_empty(shape)
+        h_p = h.data_ptr()
+    z, z_p, z_sb, z_ss = normed, 0, S * C, C
+    if normed is not None:
+        _expect(normed, "residual_norm", "normed", _F16, index)
+        z_sb, z_ss = _written_rows(normed, "normed", shape, B, S, C)
+        z_p = normed.data_ptr()
+        if z_p == x_p or z_p == h_p or (z_p == y_p and (z_sb, z_ss) != (y_sb, y_ss)):
+            raise KatzError("residual_norm: normed may be y (with the same strides), not x or out")
+    elif pre is not None:
+        z = x.new_empty(shape, dtype=_F16)
+        z_p = z.data_ptr()
+    if B and S:
+        _call_on(index, "katz_residual_norm_f16", _RESIDUAL_NORM_ARGS.pack(
+            x_p, y_p, gate_p, scale_p, shift_p, post_w, post_b, pre_w, pre_b, h_p, z_p, x_sb, x_ss, y_sb, y_ss, h_sb, h_ss, z_sb, z_ss,
+            gate_sb, gate_ss, scale_sb, scale_ss, shift_sb, shift_ss, B, S, C, 0 if dtype is _F16 else 1, post_kind, pre_kind, post_eps, pre_eps,
+            residual_scale))
     return h, z
 
 

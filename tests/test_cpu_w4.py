@@ -45,8 +45,13 @@ def test_residual_norm_refuses_bad_arguments_without_a_device():
 
 
 def test_struct_mirrors_the_header():
-    from katz_b200 import _lib
+    from katz_b200 import _lib, ops
     assert ctypes.sizeof(_lib.ResidualNormArgs) == 11 * 8 + 14 * 8 + 6 * 4 + 3 * 4 + 4      # padded to 8
+    # the packed form that the wrapper passes is the same record
+    packed = ops._RESIDUAL_NORM_ARGS.pack(*range(1, 32), 0.25, 0.5, 0.75)
+    a = _lib.ResidualNormArgs.from_buffer_copy(packed)
+    values = [getattr(a, n) for n, _ in a._fields_]
+    assert values == list(range(1, 32)) + [0.25, 0.5, 0.75]
 
 
 def test_wrappers_refuse_cpu_tensors_and_bad_norms():
