@@ -1,4 +1,6 @@
 // 4-bit weights with group scales (w4.cuh has the format): made from fp16 weights, read back, and multiplied with few rows.
+#include <algorithm>
+
 #include "w4.cuh"
 #include "katz_b200.h"
 
@@ -122,101 +124,270 @@ __global__ void __launch_bounds__(256) dequantize_w4_kernel(const unsigned char*
 // ---------------------------------------------------------------------------------------------------------------------
 // Few rows: out[M, N] = (act(x W^T + bias) + residual) * out_scale with W in 4 bits.
 //
-// A CTA owns 16 * RT weight rows and 8 * MT rows of x; its warps take turns over blocks of 128 k. In a block a lane (g =
-// lane / 4, t = lane % 4) reads 16 bytes of weight row g and of row g + 8 (the 32 k from 32 t on), which are its operand
-// fragments of eight m16n8k16 products: the sum over k may be taken in any order as long as both operands use the same one,
-// so nothing is rearranged in memory, a lane's 32 weights lie in one group, and the pairs (k, k + 4) that the unpacking
-// gives are matched by pairing x with a byte permute. The warps' sums meet in shared memory, added in warp order.
-constexpr int W4_ROWS_WARPS = 8;
+// Bound by the stream of codes from HBM and, close behind, by the instructions that turn codes into operands; so scales, x and
+// the loop's bookkeeping are kept out of those.
+// A CTA owns 16 * RT weight rows and up to 8 * MT rows of x; its warps take turns over blocks of 128 k. Lane (g = lane / 4, t =
+// lane % 4) holds the codes of weight rows g and g + 8 as four words of eight k; a word of each row makes the A operands of two
+// m16n8k16 products. The sum over k may be taken in any order as long as both operands use the same one, so the codes are used
+// as they lie in memory, and x is laid out to match once per CTA, in shared memory: the pairs (k, k + 4) that the unpacking
+// gives, 16 bytes a lane and word, no two lanes in one bank. Which k a lane's words cover is chosen by the group size so that
+// the four lanes of a row stay inside ONE group (a lane reads 16, 8 or 4 bytes at a time): a group's products are integers
+// times x, exactly, and its scale multiplies the fp32 sum. CTAs are persistent. Each warp streams its codes through a ring in
+// shared memory with asynchronous copies, across row tiles, every lane reading back what it copied itself: the bytes in
+// flight that HBM needs (some 45 KB an SM) do not fit in registers (one block ahead in registers: 2.8 TB/s). Scales and zero
+// points of a tile lie in shared memory, read row by row while the tile before is multiplied: gathered by the lanes that use
+// them they took more tag lookups than the codes. The warps' sums meet in shared memory, added in warp order.
+constexpr int W4_ROWS_THREADS = 512;
+constexpr int W4_RING = 4;                    // blocks of a warp in flight or in use
 
-template <int MT, int RT, bool XALIGNED>
-__global__ void __launch_bounds__(W4_ROWS_WARPS * 32) linear_w4_rows_kernel(const W4Params p) {
-    __shared__ float red[W4_ROWS_WARPS][8 * MT][16 * RT + 4];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int n0 = blockIdx.x * 16 * RT, m0 = blockIdx.y * 8 * MT;
-    float acc[RT][MT][4] = {};
-    pdl_wait();
-    pdl_launch_dependents();
-    const int blocks = (p.K + 127) / 128;
-    for (int kb = warp; kb < blocks; kb += W4_ROWS_WARPS) {
-        const int k = kb * 128 + 32 * t;
-        const bool k_in = k < p.K;      // K is a multiple of 32: a lane's 32 k exist together or not at all
-        uint4 a[RT][2];
-        Group grp[RT][2];
-#pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const int n = min(n0 + 16 * r + 8 * s + g, p.N - 1);      // rows past the last are computed and not stored
-                a[r][s] = make_uint4(0, 0, 0, 0);
-                unsigned short sb = 0;
-                int z = 8;
-                if (k_in) {
-                    a[r][s] = __ldg(reinterpret_cast<const uint4*>(p.q + (size_t)n * (p.K / 2) + k / 2));
-                    const size_t j = (size_t)n * p.J + (k >> p.group_shift);
-                    sb = __ldg(p.scale + j);
-                    if (p.zero) z = __ldg(p.zero + j);
-                }
-                grp[r][s] = make_group(sb, z);
-            }
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            uint32_t b[MT][4];
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const int m = m0 + 8 * i + g;
-                uint4 xv = make_uint4(0, 0, 0, 0);
-                if (k_in && m < p.M) {
-                    const __half* src = p.x + m * p.ldx + k + 8 * c;
-                    if (XALIGNED) {
-                        xv = *reinterpret_cast<const uint4*>(src);
-                    } else {
-                        const unsigned short* e = reinterpret_cast<const unsigned short*>(src);
-                        xv = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16,
-                                        e[6] | (uint32_t)e[7] << 16);
-                    }
-                }
-                b[i][0] = __byte_perm(xv.x, xv.z, 0x5410);
-                b[i][1] = __byte_perm(xv.x, xv.z, 0x7632);
-                b[i][2] = __byte_perm(xv.y, xv.w, 0x5410);
-                b[i][3] = __byte_perm(xv.y, xv.w, 0x7632);
-            }
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                uint32_t lo[4], hi[4];
-                weights8(c == 0 ? a[r][0].x : c == 1 ? a[r][0].y : c == 2 ? a[r][0].z : a[r][0].w, grp[r][0], lo);
-                weights8(c == 0 ? a[r][1].x : c == 1 ? a[r][1].y : c == 2 ? a[r][1].z : a[r][1].w, grp[r][1], hi);
-                const uint32_t a0[4] = {lo[0], hi[0], lo[1], hi[1]}, a1[4] = {lo[2], hi[2], lo[3], hi[3]};
-#pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    mma_f16_16816(acc[r][i], a0, b[i]);
-                    mma_f16_16816(acc[r][i], a1, b[i] + 2);
-                }
-            }
-        }
-    }
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) red[warp][8 * i + 2 * t + (e & 1)][16 * r + g + 8 * (e >> 1)] = acc[r][i][e];
-    __syncthreads();
-    for (int i = threadIdx.x; i < 8 * MT * 16 * RT; i += W4_ROWS_WARPS * 32) {
-        const int ml = i / (16 * RT), nl = i % (16 * RT), m = m0 + ml, n = n0 + nl;
-        if (m >= p.M || n >= p.N) continue;
-        float v = 0.f;
-#pragma unroll
-        for (int w = 0; w < W4_ROWS_WARPS; ++w) v += red[w][ml][nl];
-        p.out[m * p.ldo + n] = __float2half_rn(w4_epilogue(p, v, m, n));
-    }
+// 16, 8 or 4 bytes of codes, global -> shared, zeros if !in. L2 fetches the 256 bytes around them, most of which the CTA's
+// other warps are about to ask for: a row at a time a warp reads 64 bytes, and HBM gives such pieces at half its rate.
+template <int BYTES>
+__device__ __forceinline__ void copy_codes(uint32_t dst, const unsigned char* src, bool in) {
+    const int n = in ? BYTES : 0;
+    if (BYTES == 16) asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+    else asm volatile("cp.async.ca.shared.global.L2::256B [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(n), "n"(BYTES) : "memory");
 }
 
-template <int MT, int RT>
-static void launch_rows(const W4Params& p, bool xaligned, cudaStream_t st) {
-    const dim3 grid(ceil_div(p.N, 16 * RT), ceil_div(p.M, 8 * MT));
-    if (xaligned) launch_k(linear_w4_rows_kernel<MT, RT, true>, grid, W4_ROWS_WARPS * 32, 0, st, p);
-    else launch_k(linear_w4_rows_kernel<MT, RT, false>, grid, W4_ROWS_WARPS * 32, 0, st, p);
+// stride of a row of scales in shared memory: an odd number of 4-byte words, so that eight rows lie in different banks
+static __host__ __device__ inline int scale_stride(int J) { return (J + 1) / 2 % 2 ? (J + 1) / 2 * 2 : (J + 1) / 2 * 2 + 2; }
+// bytes of a row of x in shared memory: neighbouring rows 64 bytes apart modulo 128
+static __host__ __device__ inline int x_row_bytes(int K) { return (K + 127) / 128 * 256 + 64; }
+
+// where word i of lane t lies in a block of 128 k, and the reverse for a multiple of eight k
+template <int GROUP>
+struct Words {
+    static constexpr int GROUPS = 128 / GROUP, PER_GROUP = 4 / GROUPS;      // groups a block, words a group
+    static __device__ __forceinline__ int k(int i, int t) { return (i / PER_GROUP) * GROUP + t * (8 * PER_GROUP) + 8 * (i % PER_GROUP); }
+    static __device__ __forceinline__ int slot(int k) {      // 4 i + t
+        const int r = k % GROUP;
+        return 4 * ((k / GROUP) * PER_GROUP + r / 8 % PER_GROUP) + r / (8 * PER_GROUP);
+    }
+};
+
+// eight values of x as the pairs (0,4), (1,5), (2,6), (3,7)
+__device__ __forceinline__ uint4 load_x_pairs(const __half* src, bool aligned) {
+    uint4 v;
+    if (aligned) {
+        v = *reinterpret_cast<const uint4*>(src);
+    } else {
+        const unsigned short* e = reinterpret_cast<const unsigned short*>(src);
+        v = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
+    }
+    return make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
+                      __byte_perm(v.y, v.w, 0x7632));
+}
+
+template <int MT, int GROUP, bool ZERO>
+__global__ void __launch_bounds__(W4_ROWS_THREADS) linear_w4_rows_kernel(const W4Params p, int rows_per_cta, bool xaligned) {
+    typedef Words<GROUP> W;
+    extern __shared__ __align__(16) unsigned char rows_smem[];
+    constexpr int LD = 16 + 4;
+    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int m0 = blockIdx.y * rows_per_cta, rows = min(rows_per_cta, p.M - m0);
+    const int sld = scale_stride(p.J), blocks = (p.K + 127) / 128, xld = x_row_bytes(p.K), tiles = (p.N + 15) / 16;
+    unsigned char* xs = rows_smem;                                                        // [rows][xld]
+    unsigned char* ring = xs + rows_per_cta * xld;                                        // [warp][W4_RING][2 rows][lane][16 bytes]
+    float* red = reinterpret_cast<float*>(ring + warps * W4_RING * 1024);                 // [warp][8 * MT][LD]
+    unsigned short* scales = reinterpret_cast<unsigned short*>(red + warps * 8 * MT * LD);      // [2][16][sld]
+    unsigned char* zeros = reinterpret_cast<unsigned char*>(scales + 2 * 16 * sld);             // [2][16][sld]
+    const uint32_t mine_at = smem_u32(ring) + warp * W4_RING * 1024 + lane * 16;
+    // the next block to copy: of this warp's blocks of tile ctile the one at ck, whose codes of this lane lie at src[]
+    int ctile = blockIdx.x, ck = warp;
+    uint32_t cslot = 0;
+    const unsigned char* src[2];
+    auto at_tile = [&]() {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)      // rows past the last are computed and not stored
+            src[h] = p.q + (size_t)min(ctile * 16 + 8 * h + g, p.N - 1) * (p.K / 2) + warp * 64 + 4 * W::PER_GROUP * t;
+    };
+    at_tile();
+    auto copy_next = [&]() {
+        if (ctile < tiles) {
+            // K is a multiple of 32: all of what a lane copies at a time exists, or none (only the last block lacks any)
+            const int left = p.K - ck * 128;
+#pragma unroll
+            for (int j = 0; j < W::GROUPS; ++j) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t dst = mine_at + cslot + h * 512 + j * 4 * W::PER_GROUP;
+                    if (left >= 128) copy_codes<4 * W::PER_GROUP>(dst, src[h] + j * (GROUP / 2), true);
+                    else {
+                        const bool in = W::k(j * W::PER_GROUP, t) < left;
+                        copy_codes<4 * W::PER_GROUP>(dst, in ? src[h] + j * (GROUP / 2) : p.q, in);
+                    }
+                }
+            }
+            ck += warps;
+            src[0] += warps * 64;
+            src[1] += warps * 64;
+            if (ck >= blocks) {
+                ck = warp;
+                ctile += gridDim.x;
+                at_tile();
+            }
+        }
+        cp_async_commit();
+        cslot = (cslot + 1024) % (W4_RING * 1024);
+    };
+    auto read_scales = [&](int tile, int buf) {
+        for (int r = warp; r < 16; r += warps) {
+            const size_t at = (size_t)min(tile * 16 + r, p.N - 1) * p.J;
+            for (int j = lane; j < p.J; j += 32) {
+                scales[(buf * 16 + r) * sld + j] = __ldg(p.scale + at + j);
+                if (ZERO) zeros[(buf * 16 + r) * sld + j] = __ldg(p.zero + at + j);
+            }
+        }
+    };
+    pdl_wait();
+    pdl_launch_dependents();
+#pragma unroll
+    for (int i = 0; i < W4_RING - 1; ++i) copy_next();
+    read_scales(blockIdx.x, 0);
+    for (int v = threadIdx.x; v < blocks * 16; v += blockDim.x) {
+        const int k = v * 8;
+        for (int m = 0; m < rows; ++m)
+            *reinterpret_cast<uint4*>(xs + m * xld + (k / 128 * 16 + W::slot(k % 128)) * 16) =
+                k < p.K ? load_x_pairs(p.x + (m0 + m) * p.ldx + k, xaligned) : make_uint4(0, 0, 0, 0);
+    }
+    __syncthreads();
+    // columns of x past the last row hold another row: what they give is not stored
+    const uint32_t x_mine = smem_u32(xs) + 16 * t;
+    uint32_t x_row[MT];
+#pragma unroll
+    for (int c = 0; c < MT; ++c) x_row[c] = x_mine + min(8 * c + g, rows - 1) * xld;
+    uint32_t slot = 0;
+    int buf = 0;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, buf ^= 1) {
+        if (tile + (int)gridDim.x < tiles) read_scales(tile + gridDim.x, buf ^ 1);      // seen after this tile's barriers
+        const unsigned short* s_row = scales + (buf * 16 + g) * sld;
+        const unsigned char* z_row = zeros + (buf * 16 + g) * sld;
+        float acc[MT][4] = {};
+        for (int kb = warp; kb < blocks; kb += warps) {
+            cp_async_wait<W4_RING - 2>();
+            const uint4 v4[2] = {lds128(mine_at + slot), lds128(mine_at + slot + 512)};
+            slot = (slot + 1024) % (W4_RING * 1024);
+            copy_next();      // into the slot that was read in the round before
+            const uint32_t v[2][4] = {{v4[0].x, v4[0].y, v4[0].z, v4[0].w}, {v4[1].x, v4[1].y, v4[1].z, v4[1].w}};
+#pragma unroll
+            for (int j = 0; j < W::GROUPS; ++j) {
+                float part[MT][2][4];      // two chains of products
+                const int jg = min(kb * W::GROUPS + j, p.J - 1);      // past the last k x is zero
+                __half2 low[2], high[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    low[h] = as_half2(0xe408e408u);       // -(1024 + 8)
+                    high[h] = as_half2(0xd480d480u);      // -(64 + 8)
+                    if (ZERO) {
+                        const uint32_t z = z_row[8 * h * sld + jg];
+                        low[h] = as_half2(0xe400e400u + z * 0x00010001u);
+                        high[h] = as_half2(0xd400d400u + z * 0x00100010u);
+                    }
+                }
+#pragma unroll
+                for (int i = j * W::PER_GROUP; i < (j + 1) * W::PER_GROUP; ++i) {
+                    __half2 lo[4], hi[4];
+                    unpack8(v[0][i], low[0], high[0], lo);
+                    unpack8(v[1][i], low[1], high[1], hi);
+                    const uint32_t a0[4] = {as_u32(lo[0]), as_u32(hi[0]), as_u32(lo[1]), as_u32(hi[1])};
+                    const uint32_t a1[4] = {as_u32(lo[2]), as_u32(hi[2]), as_u32(lo[3]), as_u32(hi[3])};
+#pragma unroll
+                    for (int c = 0; c < MT; ++c) {
+                        const uint4 b = lds128(x_row[c] + (kb * 4 + i) * 64);
+                        const uint32_t b0[2] = {b.x, b.y}, b1[2] = {b.z, b.w};
+                        if (i % W::PER_GROUP == 0) {
+                            mma_f16_16816_first(part[c][0], a0, b0);
+                            mma_f16_16816_first(part[c][1], a1, b1);
+                        } else {
+                            mma_f16_16816(part[c][0], a0, b0);
+                            mma_f16_16816(part[c][1], a1, b1);
+                        }
+                    }
+                }
+                const float sl = bf16_bits_to_float(s_row[jg]), sh = bf16_bits_to_float(s_row[8 * sld + jg]);
+#pragma unroll
+                for (int c = 0; c < MT; ++c)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[c][e] = fmaf(e < 2 ? sl : sh, part[c][0][e] + part[c][1][e], acc[c][e]);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < MT; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) red[(warp * 8 * MT + 8 * c + 2 * t + (e & 1)) * LD + g + 8 * (e >> 1)] = acc[c][e];
+        __syncthreads();
+        for (int i = threadIdx.x; i < rows * 16; i += blockDim.x) {
+            const int ml = i / 16, nl = i % 16, n = tile * 16 + nl;
+            const long long m = m0 + ml;
+            if (n >= p.N) continue;
+            float v = 0.f;
+            for (int w = 0; w < warps; ++w) v += red[(w * 8 * MT + ml) * LD + nl];
+            if (p.bias) v += __half2float(p.bias[n]);
+            if (p.act == KATZ_ACT_SILU) v = silu_f(v);
+            if (p.residual) v += __half2float(p.residual[m * p.ldr + n]);
+            p.out[m * p.ldo + n] = __float2half_rn(v * p.out_scale);
+        }
+        __syncthreads();
+    }
+    cp_async_wait<0>();
+}
+
+static int sm_count() {
+    static int n[KATZ_MAX_DEVICES] = {};
+    int& c = n[current_device_index()];
+    if (!c) {
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&c, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || c <= 0) c = 148;
+    }
+    return c;
+}
+
+struct RowsLaunch {
+    int rows, warps;      // of x a CTA
+    size_t smem;
+};
+// false: K is too long for even one row of x and its scales in shared memory
+static bool rows_launch(const W4Params& p, RowsLaunch& l) {
+    const int mt = p.M <= 8 ? 1 : 2, blocks = ceil_div(p.K, 128);
+    for (int most = 8; most <= W4_ROWS_THREADS / 32; most += 8) {
+        // as many warps as share the blocks of k evenly
+        l.warps = ceil_div(blocks, ceil_div(blocks, most));
+        const long long fixed = (long long)l.warps * (W4_RING * 1024 + 8 * mt * 20 * 4) + 2ll * 16 * scale_stride(p.J) * (p.zero ? 3 : 2);
+        const long long fit = (232448 - fixed) / x_row_bytes(p.K);
+        if (fixed >= 232448 || fit < 1) return false;
+        l.rows = (int)std::min<long long>(std::min(p.M, 8 * mt), fit);
+        l.smem = (size_t)(fixed + (long long)l.rows * x_row_bytes(p.K));
+        // Eight warps a CTA where four such CTAs fit an SM: what a tile costs outside its blocks (barriers, sums, scales) is
+        // spread over twice as many of them. With more x in shared memory, or too few tiles to go round, sixteen.
+        if (4 * (l.smem + 1024) <= 233472 && ceil_div(p.N, 16) >= 2 * sm_count()) break;
+    }
+    return true;
+}
+
+template <int MT, int GROUP>
+static int launch_rows(const W4Params& p, const RowsLaunch& l, bool xaligned, cudaStream_t st) {
+    const int row_blocks = ceil_div(p.M, l.rows);
+    KATZ_CHECK_ARG(row_blocks <= 65535, KATZ_ESIZE);
+    auto kernel = p.zero ? linear_w4_rows_kernel<MT, GROUP, true> : linear_w4_rows_kernel<MT, GROUP, false>;
+    static bool attr_dev[KATZ_MAX_DEVICES][2] = {};
+    bool& attr = attr_dev[current_device_index()][p.zero != nullptr];
+    if (!attr) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
+        if (e != cudaSuccess) return (int)e;
+        attr = true;
+    }
+    // resident CTAs: 228 KB of shared memory an SM (1 KB of it per CTA), 64 registers a thread
+    const int per_sm = std::max(1, std::min(1024 / (l.warps * 32), (int)(233472 / (l.smem + 1024))));
+    const int slots = std::max(1, sm_count() * per_sm / row_blocks);
+    launch_k(kernel, dim3(std::min(ceil_div(p.N, 16), slots), row_blocks), l.warps * 32, l.smem, st, p, l.rows, xaligned);
+    KATZ_LAUNCH_RET();
+}
+
+template <int MT>
+static int launch_rows(const W4Params& p, const RowsLaunch& l, bool xaligned, cudaStream_t st) {
+    if (p.group_shift == 5) return launch_rows<MT, 32>(p, l, xaligned, st);
+    if (p.group_shift == 6) return launch_rows<MT, 64>(p, l, xaligned, st);
+    return launch_rows<MT, 128>(p, l, xaligned, st);
 }
 
 static int group_shift_of(int group) { return group == 32 ? 5 : group == 64 ? 6 : group == 128 ? 7 : -1; }
@@ -273,12 +444,11 @@ extern "C" int katz_linear_w4_f16(const void* x, long long ldx, const void* q, c
     p.ldx = ldx; p.ldo = ldo; p.ldr = ldr;
     p.M = M; p.N = N; p.K = K; p.J = ceil_div(K, group); p.group_shift = shift;
     p.act = act; p.out_scale = out_scale;
-    KATZ_CHECK_ARG(ceil_div(M, 32) <= 65535, KATZ_ESIZE);
     const bool xaligned = aligned16(x) && (M == 1 || ldx % 8 == 0);
     cudaStream_t st = (cudaStream_t)stream;
-    if (M > 16 && xaligned && K >= W4_TC05_MIN_K) return linear_w4_tc05(p, st);
-    if (M <= 8) launch_rows<1, 1>(p, xaligned, st);
-    else if (M <= 16) launch_rows<2, 1>(p, xaligned, st);
-    else launch_rows<4, 2>(p, xaligned, st);
-    KATZ_LAUNCH_RET();
+    RowsLaunch l;
+    const bool rows = rows_launch(p, l), tc05 = xaligned && K >= W4_TC05_MIN_K;
+    if (tc05 && (M > 16 || !rows)) return linear_w4_tc05(p, st);
+    KATZ_CHECK_ARG(rows, KATZ_ESIZE);
+    return M <= 8 ? launch_rows<1>(p, l, xaligned, st) : launch_rows<2>(p, l, xaligned, st);
 }

@@ -62,6 +62,13 @@ __device__ __forceinline__ void weights8(uint32_t w, const Group& g, uint32_t* o
     for (int e = 0; e < 4; ++e) o[e] = as_u32(__hmul2(d[e], g.scale));
 }
 
+// 16 bytes of shared memory by 32-bit address
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+
 }  // namespace w4
 
 struct W4Params {
@@ -77,14 +84,6 @@ struct W4Params {
     int act;
     float out_scale;
 };
-
-__device__ __forceinline__ float w4_epilogue(const W4Params& p, float acc, int m, int n) {
-    float v = acc * w4::OPERAND_UNSCALE;
-    if (p.bias) v += __half2float(p.bias[n]);
-    if (p.act == KATZ_ACT_SILU) v = silu_f(v);
-    if (p.residual) v += __half2float(p.residual[m * p.ldr + n]);
-    return v * p.out_scale;
-}
 
 // The product for more rows on the tcgen05 path (w4_tc05.cu): p.x 16-byte aligned with ldx % 8 == 0, K >= W4_TC05_MIN_K.
 constexpr int W4_TC05_MIN_K = 128;

@@ -69,11 +69,6 @@ __device__ __forceinline__ void weights8_in_order(uint32_t w, __half2 minus, __h
 
 // Shared memory by 32-bit address: the aligned base of dynamic shared memory is an integer to the compiler, and through a
 // pointer made of it every access would be a generic one with 64-bit arithmetic.
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-    return v;
-}
 __device__ __forceinline__ uint32_t lds16(uint32_t a) {
     unsigned short v;
     asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
