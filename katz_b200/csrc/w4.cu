@@ -1,6 +1,7 @@
 // 4-bit weights with group scales (w4.cuh has the format): made from fp16 weights, read back, and multiplied with few rows.
 #include <algorithm>
 
+#include "tc05.cuh"      // packed fp32 arithmetic
 #include "w4.cuh"
 #include "katz_b200.h"
 
@@ -15,110 +16,132 @@ using namespace w4;
 // that is comes out exact. |w / scale| <= 7 * (1 + 2^-8): no code leaves 1..15.
 // A group that holds an infinity or a NaN gets a NaN scale: what is read back of it is NaN, never a plausible number.
 //
-// Bound by HBM (2.5 bytes per weight and the scales). A lane holds 8 weights; a group is 4, 8 or 16 neighbouring lanes; a
-// warp works on W4_PIECES pieces of 256 weights at a time so that enough loads are in flight.
+// Bound by HBM (2.5 bytes per weight and the scales), which leaves about ten instructions a weight. A lane holds 8 weights; a
+// group is 4, 8 or 16 neighbouring lanes; a warp works on W4_PIECES pieces of 256 weights so that enough loads are in flight.
+// FLAT (contiguous rows of whole groups): the matrix is one run of groups and no lane is idle at a row's end.
 constexpr int W4_PIECES = 4;
 
 __device__ __forceinline__ __half2 hmax2_abs_nan(__half2 a, __half2 b) { return __hmax2_nan(__habs2(a), __habs2(b)); }
 
-template <int GROUP>
+// piece i of this warp: the row and k of this lane's 8 weights (FLAT: row 0, k over the whole matrix)
+template <bool FLAT>
+struct Piece {
+    long long row, k;
+    bool in;
+    __device__ __forceinline__ Piece(uint32_t index, uint32_t total, uint32_t pieces_per_row, long long K, int lane) {
+        row = FLAT ? 0 : index / pieces_per_row;
+        k = (long long)(FLAT ? index : index - (uint32_t)row * pieces_per_row) * 256 + lane * 8;
+        in = index < total && k < K;
+    }
+};
+
+template <int GROUP, bool FLAT>
 __global__ void __launch_bounds__(256) quantize_w4_kernel(const __half* __restrict__ w, long long ldw, unsigned char* __restrict__ q,
-                                                          unsigned short* __restrict__ scale, int N, int K, int J,
-                                                          int pieces_per_row) {
+                                                          unsigned short* __restrict__ scale, long long K, int J, uint32_t total,
+                                                          uint32_t pieces_per_row) {
     pdl_wait();      // writes weights: the next kernel is not released early
     constexpr int LANES = GROUP / 8;
     const int lane = threadIdx.x & 31;
-    const long long total = (long long)N * pieces_per_row;
-    const long long first = ((long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * W4_PIECES;
-    long long row = first / pieces_per_row;
-    int piece = (int)(first - row * pieces_per_row);
+    const uint32_t first = (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * W4_PIECES;
     uint4 v[W4_PIECES];
-    long long rows[W4_PIECES];
-    int ks[W4_PIECES];
 #pragma unroll
     for (int i = 0; i < W4_PIECES; ++i) {
-        rows[i] = first + i < total ? row : -1;
-        ks[i] = piece * 256 + lane * 8;
+        const Piece<FLAT> at(first + i, total, pieces_per_row, K, lane);
         v[i] = make_uint4(0, 0, 0, 0);
-        if (rows[i] >= 0 && ks[i] < K) v[i] = __ldg(reinterpret_cast<const uint4*>(w + row * ldw + ks[i]));
-        if (++piece == pieces_per_row) {
-            piece = 0;
-            ++row;
-        }
+        if (at.in) v[i] = __ldg(reinterpret_cast<const uint4*>(w + at.row * ldw + at.k));
     }
 #pragma unroll
     for (int i = 0; i < W4_PIECES; ++i) {
-        if (rows[i] < 0) return;      // uniform over the warp
+        if (first + i >= total) return;      // uniform over the warp
         const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
         __half2 m2 = hmax2_abs_nan(hmax2_abs_nan(as_half2(u[0]), as_half2(u[1])), hmax2_abs_nan(as_half2(u[2]), as_half2(u[3])));
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) m2 = hmax2_abs_nan(m2, as_half2(__shfl_xor_sync(0xffffffffu, as_u32(m2), o)));
         const float top = __half2float(__hmax_nan(__low2half(m2), __high2half(m2)));
-        __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(top, 7.0f));
+        // top / 7 rounded once (a product and one residual step), then to bf16: 11 bits over 7 are never so near the middle of
+        // two bf16 numbers that the first rounding decides, unless they are exactly there
+        float s7 = top * (1.0f / 7.0f);
+        s7 = fmaf(fmaf(-7.0f, s7, top), 1.0f / 7.0f, s7);
+        __nv_bfloat16 sb = __float2bfloat16_rn(s7);
         if (!(top <= 65504.0f)) sb = __float2bfloat16_rn(__uint_as_float(0x7fc00000u));
         const float s = __bfloat162float(sb);
-        const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
-        uint32_t codes = 0;
+        float inv;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+        if (!(s > 0.f)) inv = 0.f;
+        const float2 inv2 = make_float2(inv, inv), s2 = make_float2(-s, -s), magic = make_float2(12582912.0f, 12582912.0f);
+        // Adding 1.5 * 2^23 rounds to an integer n (ties to even) and leaves 0x4b400000 + n as the float's bits. Summed with
+        // weights 16^e they are the eight n in base 16, plus a constant; 8 is the code of zero.
+        uint32_t codes = 0x88888888u - 0x4b400000u * 0x11111111u;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float2 f = unpack_half2(u[e]);
-            float t0 = f.x * inv, t1 = f.y * inv;
-            t0 = fmaf(fmaf(-t0, s, f.x), inv, t0);
-            t1 = fmaf(fmaf(-t1, s, f.y), inv, t1);
-            // adding 1.5 * 2^23 rounds to an integer (ties to even) and leaves it in the low bits; 8 is the code of zero
-            const uint32_t c0 = __float_as_uint(t0 + 12582912.0f) + 8u, c1 = __float_as_uint(t1 + 12582912.0f) + 8u;
-            codes |= ((c0 & 15u) | ((c1 & 15u) << 4)) << (8 * e);
+            float2 t = tc05::mul2(f, inv2);
+            t = tc05::fma2(tc05::fma2(t, s2, f), inv2, t);
+            t = tc05::add2(t, magic);
+            codes += (__float_as_uint(t.x) << (8 * e)) + (__float_as_uint(t.y) << (8 * e + 4));
         }
-        if (ks[i] < K) {
-            *reinterpret_cast<uint32_t*>(q + rows[i] * (K / 2) + ks[i] / 2) = codes;
-            if ((lane & (LANES - 1)) == 0) scale[rows[i] * J + ks[i] / GROUP] = __bfloat16_as_ushort(sb);
+        const Piece<FLAT> at(first + i, total, pieces_per_row, K, lane);
+        if (at.in) {
+            *reinterpret_cast<uint32_t*>(q + at.row * (K / 2) + at.k / 2) = codes;
+            if ((lane & (LANES - 1)) == 0) scale[at.row * J + at.k / GROUP] = __bfloat16_as_ushort(sb);
         }
     }
 }
 
 // codes, scales -> fp16(scale * (code - zero)), one rounding. Bound by HBM (2.5 bytes per weight); the same shape as above.
+template <int GROUP, bool FLAT>
 __global__ void __launch_bounds__(256) dequantize_w4_kernel(const unsigned char* __restrict__ q, const unsigned short* __restrict__ scale,
                                                             const unsigned char* __restrict__ zero, __half* __restrict__ w,
-                                                            long long ldw, int N, int K, int J, int group_shift, int pieces_per_row) {
+                                                            long long ldw, long long K, int J, uint32_t total, uint32_t pieces_per_row) {
     pdl_wait();      // writes weights: the next kernel is not released early
     const int lane = threadIdx.x & 31;
-    const long long total = (long long)N * pieces_per_row;
-    const long long first = ((long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * W4_PIECES;
-    long long row = first / pieces_per_row;
-    int piece = (int)(first - row * pieces_per_row);
+    const uint32_t first = (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * W4_PIECES;
     uint32_t v[W4_PIECES];
     unsigned short sb[W4_PIECES];
     unsigned char zb[W4_PIECES];
-    __half* dst[W4_PIECES];
 #pragma unroll
     for (int i = 0; i < W4_PIECES; ++i) {
-        const int k = piece * 256 + lane * 8;
-        const bool in = first + i < total && k < K;
-        dst[i] = in ? w + row * ldw + k : nullptr;
-        v[i] = in ? __ldg(reinterpret_cast<const uint32_t*>(q + row * (K / 2) + k / 2)) : 0u;
-        sb[i] = in ? __ldg(scale + row * J + (k >> group_shift)) : (unsigned short)0;
-        zb[i] = in && zero ? __ldg(zero + row * J + (k >> group_shift)) : (unsigned char)8;
-        if (++piece == pieces_per_row) {
-            piece = 0;
-            ++row;
+        const Piece<FLAT> at(first + i, total, pieces_per_row, K, lane);
+        v[i] = 0;
+        sb[i] = 0;
+        zb[i] = 8;
+        if (at.in) {
+            const long long j = at.row * J + at.k / GROUP;
+            v[i] = __ldg(reinterpret_cast<const uint32_t*>(q + at.row * (K / 2) + at.k / 2));
+            sb[i] = __ldg(scale + j);
+            if (zero) zb[i] = __ldg(zero + j);
         }
     }
 #pragma unroll
     for (int i = 0; i < W4_PIECES; ++i) {
-        if (!dst[i]) continue;
+        const Piece<FLAT> at(first + i, total, pieces_per_row, K, lane);
+        if (!at.in) continue;
         __half2 d[4];
-        unpack8(v[i], __float2half2_rn((float)(-1024 - (int)zb[i])), __float2half2_rn((float)(-64 - (int)zb[i])), d);
+        unpack8(v[i], as_half2(0xe400e400u + zb[i] * 0x00010001u), as_half2(0xd400d400u + zb[i] * 0x00100010u), d);
         const float s = bf16_bits_to_float(sb[i]);
         float2 f[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            f[e] = __half22float2(d[e]);
-            f[e].x *= s;
-            f[e].y *= s;
-        }
-        *reinterpret_cast<uint4*>(dst[i]) = make_uint4(pack_half2(f[0].x, f[1].x), pack_half2(f[2].x, f[3].x), pack_half2(f[0].y, f[1].y),
-                                                       pack_half2(f[2].y, f[3].y));
+        for (int e = 0; e < 4; ++e) f[e] = tc05::mul2(__half22float2(d[e]), make_float2(s, s));
+        *reinterpret_cast<uint4*>(w + at.row * ldw + at.k) = make_uint4(pack_half2(f[0].x, f[1].x), pack_half2(f[2].x, f[3].x),
+                                                                        pack_half2(f[0].y, f[1].y), pack_half2(f[2].y, f[3].y));
     }
+}
+
+struct PieceGrid {
+    long long K;             // of a row, FLAT: of the matrix
+    uint32_t total, per_row, ctas;
+    bool flat, ok;
+};
+static PieceGrid piece_grid(int N, int K, int group, long long ldw) {
+    PieceGrid g{};
+    g.flat = (ldw == K || N == 1) && K % group == 0;
+    g.K = g.flat ? (long long)N * K : K;
+    const long long per_row = ceil_div_ll(g.K, 256), total = g.flat ? per_row : N * per_row;
+    g.per_row = (uint32_t)per_row;
+    g.total = (uint32_t)total;
+    g.ctas = (uint32_t)ceil_div_ll(total, 8 * W4_PIECES);
+    g.ok = total < (1ll << 31);
+    return g;
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -402,13 +425,13 @@ extern "C" int katz_quantize_w4_f16(const void* w, long long ldw, void* q, void*
     KATZ_CHECK_ARG(shift > 0, KATZ_EINVAL);
     KATZ_CHECK_ARG(N > 0 && K > 0 && K % 32 == 0 && ldw >= K, KATZ_ESIZE);
     KATZ_CHECK_ARG(aligned16(w) && ldw % 8 == 0 && aligned16(q) && ((uintptr_t)scale & 1) == 0, KATZ_EALIGN);
-    const int pieces = ceil_div(K, 256);
-    const long long ctas = ceil_div_ll((long long)N * pieces, 8 * W4_PIECES);
-    KATZ_CHECK_ARG(ctas < (1ll << 31), KATZ_ESIZE);
-    const int J = ceil_div(K, group);
-    auto kernel = group == 32 ? quantize_w4_kernel<32> : group == 64 ? quantize_w4_kernel<64> : quantize_w4_kernel<128>;
-    launch_k(kernel, (unsigned)ctas, 256, 0, (cudaStream_t)stream, (const __half*)w, ldw, (unsigned char*)q, (unsigned short*)scale, N, K,
-             J, pieces);
+    const PieceGrid g = piece_grid(N, K, group, ldw);
+    KATZ_CHECK_ARG(g.ok, KATZ_ESIZE);
+    auto kernel = group == 32 ? (g.flat ? quantize_w4_kernel<32, true> : quantize_w4_kernel<32, false>)
+                  : group == 64 ? (g.flat ? quantize_w4_kernel<64, true> : quantize_w4_kernel<64, false>)
+                                : (g.flat ? quantize_w4_kernel<128, true> : quantize_w4_kernel<128, false>);
+    launch_k(kernel, g.ctas, 256, 0, (cudaStream_t)stream, (const __half*)w, ldw, (unsigned char*)q, (unsigned short*)scale, g.K,
+             ceil_div(K, group), g.total, g.per_row);
     KATZ_LAUNCH_RET();
 }
 
@@ -419,11 +442,13 @@ extern "C" int katz_dequantize_w4_f16(const void* q, const void* scale, const vo
     KATZ_CHECK_ARG(shift > 0, KATZ_EINVAL);
     KATZ_CHECK_ARG(N > 0 && K > 0 && K % 32 == 0 && ldw >= K, KATZ_ESIZE);
     KATZ_CHECK_ARG(aligned16(w) && ldw % 8 == 0 && aligned16(q) && ((uintptr_t)scale & 1) == 0, KATZ_EALIGN);
-    const int pieces = ceil_div(K, 256);
-    const long long ctas = ceil_div_ll((long long)N * pieces, 8 * W4_PIECES);
-    KATZ_CHECK_ARG(ctas < (1ll << 31), KATZ_ESIZE);
-    launch_k(dequantize_w4_kernel, (unsigned)ctas, 256, 0, (cudaStream_t)stream, (const unsigned char*)q, (const unsigned short*)scale,
-             (const unsigned char*)zero, (__half*)w, ldw, N, K, ceil_div(K, group), shift, pieces);
+    const PieceGrid g = piece_grid(N, K, group, ldw);
+    KATZ_CHECK_ARG(g.ok, KATZ_ESIZE);
+    auto kernel = group == 32 ? (g.flat ? dequantize_w4_kernel<32, true> : dequantize_w4_kernel<32, false>)
+                  : group == 64 ? (g.flat ? dequantize_w4_kernel<64, true> : dequantize_w4_kernel<64, false>)
+                                : (g.flat ? dequantize_w4_kernel<128, true> : dequantize_w4_kernel<128, false>);
+    launch_k(kernel, g.ctas, 256, 0, (cudaStream_t)stream, (const unsigned char*)q, (const unsigned short*)scale, (const unsigned char*)zero,
+             (__half*)w, ldw, g.K, ceil_div(K, group), g.total, g.per_row);
     KATZ_LAUNCH_RET();
 }
 

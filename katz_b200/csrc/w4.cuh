@@ -20,20 +20,7 @@ namespace w4 {
 // of 2^-17 to 4366, and weights of 1e-5 keep their bits.
 constexpr float OPERAND_SCALE = 64.0f, OPERAND_UNSCALE = 1.0f / 64.0f;
 
-// half2 constants of one group of one row: what turns four bits into weights.
-//   (word & 0x000f000f) | 0x6400'6400 is the pair (1024 + c0, 1024 + c4) in fp16: subtracting 1024 + zero is exact;
-//   (word & 0x00f000f0) | 0x6400'6400 is (1024 + 16 c1, 1024 + 16 c5): times 1/16, minus 64 + zero, is exact too.
-struct Group {
-    __half2 scale, low, high;
-};
 __device__ __forceinline__ float bf16_bits_to_float(unsigned short b) { return __uint_as_float((uint32_t)b << 16); }
-__device__ __forceinline__ Group make_group(unsigned short scale_bits, int zero) {
-    Group g;
-    g.scale = __float2half2_rn(bf16_bits_to_float(scale_bits) * OPERAND_SCALE);
-    g.low = __float2half2_rn((float)(-1024 - zero));
-    g.high = __float2half2_rn((float)(-64 - zero));
-    return g;
-}
 __device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
@@ -45,6 +32,8 @@ __device__ __forceinline__ uint32_t and_or_1024(uint32_t w) {
     return r;
 }
 
+//   (word & 0x000f000f) | 0x6400'6400 is the pair (1024 + c0, 1024 + c4) in fp16: subtracting 1024 + zero is exact;
+//   (word & 0x00f000f0) | 0x6400'6400 is (1024 + 16 c1, 1024 + 16 c5): times 1/16, minus 64 + zero, is exact too.
 // One word (8 codes, k = 0..7) -> code - zero as four fp16 pairs (k0,k4), (k1,k5), (k2,k6), (k3,k7)
 __device__ __forceinline__ void unpack8(uint32_t w, __half2 low, __half2 high, __half2* d) {
     const __half2 sixteenth = __float2half2_rn(0.0625f);
@@ -54,14 +43,6 @@ __device__ __forceinline__ void unpack8(uint32_t w, __half2 low, __half2 high, _
     d[2] = __hadd2(as_half2(and_or_1024<0x000f000fu>(v)), low);
     d[3] = __hfma2(as_half2(and_or_1024<0x00f000f0u>(v)), sixteenth, high);
 }
-// ... -> operands (64 * weight)
-__device__ __forceinline__ void weights8(uint32_t w, const Group& g, uint32_t* o) {
-    __half2 d[4];
-    unpack8(w, g.low, g.high, d);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = as_u32(__hmul2(d[e], g.scale));
-}
-
 // 16 bytes of shared memory by 32-bit address
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
     uint4 v;
