@@ -5,13 +5,18 @@
 // LayerNorm(v) = (v - mean) / sqrt(var + eps) * weight + bias, RMSNorm(v) = v / sqrt(mean of v^2 + eps) * weight + bias; weight and
 // bias are optional, gate, scale and shift may be per channel, per sample or per token (strides of zero).
 //
-// Bound by HBM: x and y are read once, h and z written once, 8 bytes per element in fp16. A row stays in registers from the
-// load to the store; statistics are fp32, of the values before any rounding (z is computed from the unrounded h), and the
-// variance is the mean of squared differences from the mean, so a row whose mean is large loses nothing. Rows of up to 1280
-// channels belong to one warp (sums by shuffles, no barrier), longer ones to 4 or 16 warps.
-#include "common.cuh"
+// Bound by HBM: x and y are read once, h and z written once, 8 bytes per element in fp16; next by instructions, so the
+// arithmetic is packed (two fp32 lanes an instruction). A row stays in registers from the load to the store; statistics are
+// fp32, of the values before any rounding (z is computed from the unrounded h), and the variance is the mean of squared
+// differences from the mean, so a row whose mean is large loses nothing. Rows of up to 1280 channels belong to one warp (sums
+// by shuffles, no barrier), longer ones to 4 or 16 warps.
+#include "tc05.cuh"      // packed fp32 arithmetic
 
 namespace katz {
+
+using tc05::add2;
+using tc05::fma2;
+using tc05::mul2;
 
 struct ResidualNormParams {
     const void* x;
@@ -55,219 +60,198 @@ __device__ __forceinline__ float row_sum(float v, float* red, int& slot) {
     return v;
 }
 
-// channel of element e of vector i
-template <int T, bool VEC>
-__device__ __forceinline__ int channel(int i, int e, int tid) {
-    return VEC ? (i * T + tid) * 8 + e : (i * 8 + e) * T + tid;
+// A thread holds NU vectors of E consecutive channels, as pairs: eight (16 bytes of fp16) beside an fp16 stream, four beside an
+// fp32 one, so that a warp's accesses to either are contiguous. Channels past the last hold zeros; FULL: there are none.
+template <int T, int E, bool VEC>
+__device__ __forceinline__ int channel(int i, int e, int tid) {      // of element e of vector i
+    return VEC ? (i * T + tid) * E + e : (i * E + e) * T + tid;
 }
 
-template <int T, int NV, bool VEC>
-__device__ __forceinline__ void load_row(const __half* src, int C, int tid, float (&v)[NV][8]) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        if (VEC) {
-            const int c = channel<T, VEC>(i, 0, tid);
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (c < C) w = *reinterpret_cast<const uint4*>(src + c);
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 f = unpack_half2(u[e]);
-                v[i][2 * e] = f.x;
-                v[i][2 * e + 1] = f.y;
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int c = channel<T, VEC>(i, e, tid);
-                v[i][e] = c < C ? __half2float(src[c]) : 0.f;
-            }
-        }
-    }
+__device__ __forceinline__ void load_vector(const __half* p, float2 (&v)[4]) {
+    const uint4 w = *reinterpret_cast<const uint4*>(p);
+    v[0] = unpack_half2(w.x), v[1] = unpack_half2(w.y), v[2] = unpack_half2(w.z), v[3] = unpack_half2(w.w);
 }
-template <int T, int NV, bool VEC>
-__device__ __forceinline__ void load_row(const float* src, int C, int tid, float (&v)[NV][8]) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        if (VEC) {
-            const int c = channel<T, VEC>(i, 0, tid);
-            float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-            if (c < C) {
-                a = *reinterpret_cast<const float4*>(src + c);
-                b = *reinterpret_cast<const float4*>(src + c + 4);
-            }
-            const float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[i][e] = f[e];
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int c = channel<T, VEC>(i, e, tid);
-                v[i][e] = c < C ? src[c] : 0.f;
-            }
-        }
-    }
+__device__ __forceinline__ void load_vector(const __half* p, float2 (&v)[2]) {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    v[0] = unpack_half2(w.x), v[1] = unpack_half2(w.y);
 }
-template <int T, int NV, bool VEC>
-__device__ __forceinline__ void store_row(__half* dst, int C, int tid, const float (&v)[NV][8]) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        if (VEC) {
-            const int c = channel<T, VEC>(i, 0, tid);
-            if (c < C)
-                *reinterpret_cast<uint4*>(dst + c) = make_uint4(pack_half2(v[i][0], v[i][1]), pack_half2(v[i][2], v[i][3]),
-                                                                pack_half2(v[i][4], v[i][5]), pack_half2(v[i][6], v[i][7]));
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int c = channel<T, VEC>(i, e, tid);
-                if (c < C) dst[c] = __float2half_rn(v[i][e]);
-            }
-        }
-    }
+__device__ __forceinline__ void load_vector(const float* p, float2 (&v)[2]) {
+    const float4 w = *reinterpret_cast<const float4*>(p);
+    v[0] = make_float2(w.x, w.y), v[1] = make_float2(w.z, w.w);
 }
-template <int T, int NV, bool VEC>
-__device__ __forceinline__ void store_row(float* dst, int C, int tid, const float (&v)[NV][8]) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        if (VEC) {
-            const int c = channel<T, VEC>(i, 0, tid);
-            if (c < C) {
-                *reinterpret_cast<float4*>(dst + c) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
-                *reinterpret_cast<float4*>(dst + c + 4) = make_float4(v[i][4], v[i][5], v[i][6], v[i][7]);
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int c = channel<T, VEC>(i, e, tid);
-                if (c < C) dst[c] = v[i][e];
-            }
-        }
-    }
+__device__ __forceinline__ uint32_t pack(float2 v) { return pack_half2(v.x, v.y); }
+__device__ __forceinline__ void store_vector(__half* p, const float2 (&v)[4]) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack(v[0]), pack(v[1]), pack(v[2]), pack(v[3]));
+}
+__device__ __forceinline__ void store_vector(__half* p, const float2 (&v)[2]) { *reinterpret_cast<uint2*>(p) = make_uint2(pack(v[0]), pack(v[1])); }
+__device__ __forceinline__ void store_vector(float* p, const float2 (&v)[2]) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
 }
 
-// v <- normalised v (weight and bias applied)
-template <int T, int NV, bool VEC>
-__device__ __forceinline__ void normalise(float (&v)[NV][8], int kind, const __half* weight, const __half* bias, float eps, int C, int tid,
-                                          float* red, int& slot) {
-    const float inv_c = 1.0f / (float)C;
-    float mean = 0.f;
-    if (kind == KATZ_NORM_LAYER) {
-        float s = 0.f;
+template <int T_, int NU_, int E_, bool VEC_, bool FULL_>
+struct RowOf {
+    static constexpr int T = T_, NU = NU_, E = E_;
+    static constexpr bool VEC = VEC_, FULL = FULL_;
+    float2 v[NU][E / 2];
+
+    static __device__ __forceinline__ bool in(int i, int tid, int C) { return FULL || channel<T, E, VEC>(i, 0, tid) < C; }      // VEC
+    template <typename F>
+    __device__ __forceinline__ void each(F f) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NU; ++i)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s += v[i][e];      // channels past the last hold zeros
-        mean = row_sum<T>(s, red, slot) * inv_c;
+            for (int e = 0; e < E / 2; ++e) v[i][e] = f(v[i][e], i, e);
     }
-    float q = 0.f;
+    template <typename S>
+    __device__ __forceinline__ void load(const S* src, int C, int tid) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NU; ++i) {
+            if constexpr (!FULL) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float d = v[i][e] - mean;
-            if (channel<T, VEC>(i, e, tid) < C) q = fmaf(d, d, q);
+                for (int e = 0; e < E / 2; ++e) v[i][e] = make_float2(0.f, 0.f);
+            }
+            if constexpr (VEC) {
+                if (in(i, tid, C)) load_vector(src + channel<T, E, VEC>(i, 0, tid), v[i]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const int c = channel<T, E, VEC>(i, e, tid);
+                    if (c < C) (e & 1 ? v[i][e / 2].y : v[i][e / 2].x) = (float)src[c];
+                }
+            }
         }
-    const float rstd = rsqrtf(row_sum<T>(q, red, slot) * inv_c + eps);
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[i][e] = (v[i][e] - mean) * rstd;
-    if (weight) {
-        float g[NV][8];
-        load_row<T, NV, VEC>(weight, C, tid, g);
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[i][e] *= g[i][e];
     }
-    if (bias) {
-        float b[NV][8];
-        load_row<T, NV, VEC>(bias, C, tid, b);
+    template <typename S>
+    __device__ __forceinline__ void store(S* dst, int C, int tid) const {
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NU; ++i) {
+            if constexpr (VEC) {
+                if (in(i, tid, C)) store_vector(dst + channel<T, E, VEC>(i, 0, tid), v[i]);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[i][e] += b[i][e];
+                for (int e = 0; e < E; ++e) {
+                    const int c = channel<T, E, VEC>(i, e, tid);
+                    if (c < C) dst[c] = (S)(e & 1 ? v[i][e / 2].y : v[i][e / 2].x);
+                }
+            }
+        }
     }
-}
+    // v <- normalised v (weight and bias applied)
+    __device__ __forceinline__ void normalise(int kind, const __half* weight, const __half* bias, float eps, int C, int tid, float* red,
+                                              int& slot) {
+        const float inv_c = 1.0f / (float)C;
+        if (kind == KATZ_NORM_LAYER) {
+            float2 s = make_float2(0.f, 0.f);
+            each([&](float2 a, int, int) { s = add2(s, a); return a; });
+            const float mean = row_sum<T>(s.x + s.y, red, slot) * inv_c;
+            const float2 m = make_float2(-mean, -mean);
+            each([&](float2 a, int i, int e) {
+                float2 d = add2(a, m);
+                if constexpr (!FULL) {      // what lies past the last channel stays zero
+                    if (channel<T, E, VEC>(i, 2 * e, tid) >= C) d.x = 0.f;
+                    if (channel<T, E, VEC>(i, 2 * e + 1, tid) >= C) d.y = 0.f;
+                }
+                return d;
+            });
+        }
+        float2 q = make_float2(0.f, 0.f);
+        each([&](float2 a, int, int) { q = fma2(a, a, q); return a; });
+        const float rstd = rsqrtf(row_sum<T>(q.x + q.y, red, slot) * inv_c + eps);
+        const float2 r = make_float2(rstd, rstd);
+        each([&](float2 a, int, int) { return mul2(a, r); });
+        if (weight) {
+            RowOf g;
+            g.load(weight, C, tid);
+            each([&](float2 a, int i, int e) { return mul2(a, g.v[i][e]); });
+        }
+        if (bias) {
+            RowOf b;
+            b.load(bias, C, tid);
+            each([&](float2 a, int i, int e) { return add2(a, b.v[i][e]); });
+        }
+    }
+};
 
 // one row per T threads; a CTA of max(T, 128) threads
-template <int T, int NV, bool VEC, bool F32>
+template <int T, int NU, bool VEC, bool F32, bool FULL>
 __global__ void __launch_bounds__(T > 128 ? T : 128) residual_norm_kernel(const ResidualNormParams p) {
     typedef typename Stream<F32>::T XT;
+    typedef RowOf<T, NU, F32 ? 4 : 8, VEC, FULL> Row;
     __shared__ float red[2 * (T > 32 ? T / 32 : 1)];
     constexpr int ROWS = T >= 128 ? 1 : 128 / T;
     pdl_wait();
     pdl_launch_dependents();
     const int tid = threadIdx.x % T;
-    const long long row = (long long)blockIdx.x * ROWS + threadIdx.x / T;
-    if (row >= p.rows) return;      // uniform over the threads of a row
-    const long long b = row / p.S, s = row - b * p.S;
+    const uint32_t row = blockIdx.x * ROWS + threadIdx.x / T;
+    if (row >= (uint32_t)p.rows) return;      // uniform over the threads of a row
+    const uint32_t b = row / (uint32_t)p.S, s = row - b * p.S;
     int slot = 0;
-    float h[NV][8];
-    load_row<T, NV, VEC>(static_cast<const XT*>(p.x) + b * p.x_sb + s * p.x_ss, p.C, tid, h);
+    Row h;
+    h.load(static_cast<const XT*>(p.x) + b * p.x_sb + s * p.x_ss, p.C, tid);
+    const float2 scale = make_float2(p.residual_scale, p.residual_scale);
     if (p.y) {
-        float u[NV][8];
-        load_row<T, NV, VEC>(p.y + b * p.y_sb + s * p.y_ss, p.C, tid, u);
-        if (p.post_kind != KATZ_NORM_NONE) normalise<T, NV, VEC>(u, p.post_kind, p.post_w, p.post_b, p.post_eps, p.C, tid, red, slot);
+        Row u;
+        u.load(p.y + b * p.y_sb + s * p.y_ss, p.C, tid);
+        if (p.post_kind != KATZ_NORM_NONE) u.normalise(p.post_kind, p.post_w, p.post_b, p.post_eps, p.C, tid, red, slot);
         if (p.gate) {
-            float g[NV][8];
-            load_row<T, NV, VEC>(p.gate + b * p.gate_sb + s * p.gate_ss, p.C, tid, g);
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) u[i][e] *= g[i][e];
+            Row g;
+            g.load(p.gate + b * p.gate_sb + s * p.gate_ss, p.C, tid);
+            u.each([&](float2 a, int i, int e) { return mul2(a, g.v[i][e]); });
         }
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) h[i][e] = fmaf(p.residual_scale, h[i][e], u[i][e]);
+        h.each([&](float2 a, int i, int e) { return fma2(scale, a, u.v[i][e]); });
     } else {
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) h[i][e] *= p.residual_scale;
+        h.each([&](float2 a, int, int) { return mul2(a, scale); });
     }
-    if (p.h) store_row<T, NV, VEC>(static_cast<XT*>(p.h) + b * p.h_sb + s * p.h_ss, p.C, tid, h);
+    if (p.h) h.store(static_cast<XT*>(p.h) + b * p.h_sb + s * p.h_ss, p.C, tid);
     if (p.pre_kind == KATZ_NORM_NONE) return;
-    normalise<T, NV, VEC>(h, p.pre_kind, p.pre_w, p.pre_b, p.pre_eps, p.C, tid, red, slot);
+    h.normalise(p.pre_kind, p.pre_w, p.pre_b, p.pre_eps, p.C, tid, red, slot);
     if (p.scale) {
-        float g[NV][8];
-        load_row<T, NV, VEC>(p.scale + b * p.scale_sb + s * p.scale_ss, p.C, tid, g);
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) h[i][e] = fmaf(h[i][e], g[i][e], h[i][e]);
+        Row g;
+        g.load(p.scale + b * p.scale_sb + s * p.scale_ss, p.C, tid);
+        h.each([&](float2 a, int i, int e) { return fma2(a, g.v[i][e], a); });
     }
     if (p.shift) {
-        float g[NV][8];
-        load_row<T, NV, VEC>(p.shift + b * p.shift_sb + s * p.shift_ss, p.C, tid, g);
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) h[i][e] += g[i][e];
+        Row g;
+        g.load(p.shift + b * p.shift_sb + s * p.shift_ss, p.C, tid);
+        h.each([&](float2 a, int i, int e) { return add2(a, g.v[i][e]); });
     }
-    store_row<T, NV, VEC>(p.z + b * p.z_sb + s * p.z_ss, p.C, tid, h);
+    h.store(p.z + b * p.z_sb + s * p.z_ss, p.C, tid);
 }
 
-template <int T, int NV, bool VEC>
-static void launch_residual_norm(const ResidualNormParams& p, bool f32, cudaStream_t st) {
+template <int T, int NU, bool VEC, bool F32>
+static void launch_residual_norm(const ResidualNormParams& p, cudaStream_t st) {
     constexpr int ROWS = T >= 128 ? 1 : 128 / T;
     const unsigned grid = (unsigned)ceil_div_ll(p.rows, ROWS);
-    if (f32) launch_k(residual_norm_kernel<T, NV, VEC, true>, grid, T > 128 ? T : 128, 0, st, p);
-    else launch_k(residual_norm_kernel<T, NV, VEC, false>, grid, T > 128 ? T : 128, 0, st, p);
+    auto kernel = residual_norm_kernel<T, NU, VEC, F32, false>;
+    if constexpr (VEC) {
+        if (p.C == T * NU * (F32 ? 4 : 8)) kernel = residual_norm_kernel<T, NU, VEC, F32, true>;
+    }
+    launch_k(kernel, grid, T > 128 ? T : 128, 0, st, p);
 }
 
-template <bool VEC>
-static void dispatch_residual_norm(const ResidualNormParams& p, bool f32, cudaStream_t st) {
-    if (p.C <= 32 * 8) launch_residual_norm<32, 1, VEC>(p, f32, st);
-    else if (p.C <= 32 * 16) launch_residual_norm<32, 2, VEC>(p, f32, st);
-    else if (p.C <= 32 * 24) launch_residual_norm<32, 3, VEC>(p, f32, st);
-    else if (p.C <= 32 * 40) launch_residual_norm<32, 5, VEC>(p, f32, st);
-    else if (p.C <= 128 * 16) launch_residual_norm<128, 2, VEC>(p, f32, st);
-    else if (p.C <= 128 * 32) launch_residual_norm<128, 4, VEC>(p, f32, st);
-    else if (p.C <= 512 * 16) launch_residual_norm<512, 2, VEC>(p, f32, st);
-    else launch_residual_norm<512, 4, VEC>(p, f32, st);
+// T threads of up to NU vectors: the fewest vectors that hold the row
+template <int T, int NU, int MAX, bool VEC, bool F32>
+static void pick_vectors(const ResidualNormParams& p, cudaStream_t st) {
+    if constexpr (NU < MAX) {
+        if (p.C > T * NU * (F32 ? 4 : 8)) return pick_vectors<T, NU + 1, MAX, VEC, F32>(p, st);
+    }
+    launch_residual_norm<T, NU, VEC, F32>(p, st);
+}
+
+template <bool VEC, bool F32>
+static void dispatch_residual_norm(const ResidualNormParams& p, cudaStream_t st) {
+    constexpr int E = F32 ? 4 : 8, MORE = F32 ? 2 : 1;
+    if constexpr (!VEC) {      // single elements: a few sizes
+        if (p.C <= 32 * 16) launch_residual_norm<32, 2 * MORE, VEC, F32>(p, st);
+        else if (p.C <= 128 * 16) launch_residual_norm<128, 2 * MORE, VEC, F32>(p, st);
+        else launch_residual_norm<512, 4 * MORE, VEC, F32>(p, st);
+    } else if (p.C <= 32 * 5 * MORE * E) {
+        pick_vectors<32, 1, 5 * MORE, VEC, F32>(p, st);
+    } else if (p.C <= 128 * 4 * MORE * E) {
+        pick_vectors<128, 2 * MORE, 4 * MORE, VEC, F32>(p, st);
+    } else {
+        pick_vectors<512, 2 * MORE, 4 * MORE, VEC, F32>(p, st);
+    }
 }
 
 }  // namespace katz
@@ -307,7 +291,8 @@ extern "C" int katz_residual_norm_f16(const katz_residual_norm_args* a, void* st
     p.S = a->S; p.C = a->C; p.rows = rows;
     p.post_kind = a->post_kind; p.pre_kind = a->pre_kind; p.post_eps = a->post_eps; p.pre_eps = a->pre_eps;
     p.residual_scale = a->residual_scale;
-    if (vec) dispatch_residual_norm<true>(p, f32, (cudaStream_t)stream);
-    else dispatch_residual_norm<false>(p, f32, (cudaStream_t)stream);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (f32) vec ? dispatch_residual_norm<true, true>(p, st) : dispatch_residual_norm<false, true>(p, st);
+    else vec ? dispatch_residual_norm<true, false>(p, st) : dispatch_residual_norm<false, false>(p, st);
     KATZ_LAUNCH_RET();
 }
