@@ -187,9 +187,12 @@ _F16, _F32, _BF16, _U8 = torch.float16, torch.float32, torch.bfloat16, torch.uin
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _call_on(index, name, *args):
     """Launch on the current stream of CUDA device `index`, which need not be the current device."""
-    if index == torch.cuda.current_device():
+    if index == _current_device():
         call(name, *args, _raw_stream(index))
         return
     with torch.cuda.device(index):
@@ -223,7 +226,9 @@ def _w4_check(what, q, scale, zero, group):
     """(device index, N, K) of a 4-bit weight; see quantize_w4 for the format."""
     if group not in (32, 64, 128):
         raise KatzError("%s: group must be 32, 64 or 128 (got %r)" % (what, group))
-    index = _expect(q, what, "q", _U8, None)
+    index = q.get_device()
+    if q.dtype is not _U8 or index < 0:
+        _expect(q, what, "q", _U8, None)
     if q.dim() != 2 or not q.is_contiguous():
         raise KatzError("%s: q must be a contiguous [N, K/2] tensor" % what)
     N, K = q.shape
@@ -233,7 +238,8 @@ def _w4_check(what, q, scale, zero, group):
     if q.data_ptr() % 16:
         raise KatzError("%s: q must start on a 16-byte boundary" % what)
     shape = (N, (K + group - 1) // group)
-    _expect(scale, what, "scale", _BF16, index)
+    if scale.dtype is not _BF16 or scale.get_device() != index:
+        _expect(scale, what, "scale", _BF16, index)
     if scale.shape != shape or not scale.is_contiguous():
         raise KatzError("%s: scale must be a contiguous [N, ceil(K/group)] = %s tensor" % (what, shape))
     if zero is not None:
@@ -292,7 +298,8 @@ def linear_w4(x, q, scale, zero=None, group=64, bias=None, residual=None, act=AC
     `x`, `residual`, `out` may be row-strided 2-D views (unit column stride); `out` may be `residual`. Scales of 2^-23 to 64
     are covered: the weights of larger ones overflow fp16 to infinity, those of smaller ones lose bits."""
     index, N, K = _w4_check("linear_w4", q, scale, zero, group)
-    _expect(x, "linear_w4", "x", _F16, index)
+    if x.dtype is not _F16 or x.get_device() != index:
+        _expect(x, "linear_w4", "x", _F16, index)
     M = x.shape[0] if x.dim() == 2 else -1
     ldx = _row_stride(x, "linear_w4", "x", M, K)
     if act != ACT_NONE and act != ACT_SILU:
@@ -308,8 +315,9 @@ def linear_w4(x, q, scale, zero=None, group=64, bias=None, residual=None, act=AC
     bias_p = residual_p = None
     ldr = 0
     if bias is not None:
-        _expect(bias, "linear_w4", "bias", _F16, index)
-        if bias.shape != (N,) or not bias.is_contiguous():
+        if bias.dtype is not _F16 or bias.get_device() != index:
+            _expect(bias, "linear_w4", "bias", _F16, index)
+        if bias.dim() != 1 or bias.numel() != N or not bias.is_contiguous():
             raise KatzError("linear_w4: bias must be a contiguous [N] tensor")
         bias_p = bias.data_ptr()
     if residual is not None:
@@ -501,38 +509,35 @@ def _written_rows(t, name, shape, B, S, C):
 def _vector(t, name, shape, index):
     """(address, batch stride, token stride) of a gate, scale or shift: [C], [B, C] ([rows, C] for a 2-D x) or [B, S, C], sizes
     of 1 broadcast."""
-    if t is None:
-        return 0, 0, 0
-    _expect(t, "residual_norm", name, _F16, index)
+    if t.dtype is not _F16 or t.get_device() != index:
+        _expect(t, "residual_norm", name, _F16, index)
     ts, st = t.shape, t.stride()
-    d = len(ts)
-    ok = 0 < d <= len(shape) and ts[-1] == shape[-1] and (st[-1] == 1 or ts[-1] == 1)
-    strides = [0, 0]
-    first = 1 if len(shape) == 2 else 0      # a 2-D x is one batch of rows
-    for i in range(d - 1):
-        if ts[i] == 1:
-            continue
-        ok = ok and ts[i] == shape[i]
-        if not ok:
-            break
-        strides[first + i] = st[i]
+    d, full = len(ts), len(shape)
+    ok = 0 < d <= full and ts[-1] == shape[-1] and (st[-1] == 1 or ts[-1] == 1)
+    sb = ss = 0
+    if ok and d > 1:
+        if ts[0] != 1:
+            ok = ts[0] == shape[0]
+            if full == 2:      # a 2-D x is one batch of rows
+                ss = st[0]
+            else:
+                sb = st[0]
+        if d == 3 and ts[1] != 1:
+            ok = ok and ts[1] == shape[1]
+            ss = st[1]
     if not ok:
         raise KatzError("residual_norm: %s %s (strides %s) does not fit x %s" % (name, tuple(ts), st, tuple(shape)))
-    return t.data_ptr(), strides[0], strides[1]
+    return t.data_ptr(), sb, ss
 
 
-def _norm_vectors(norm, side, C, index):
-    """(kind, eps, address of weight, address of bias)"""
-    if norm is None:
-        return _lib.NORM_NONE, 0.0, 0, 0
-    at = []
-    for v in (norm.weight, norm.bias):
-        if v is not None:
-            _expect(v, "residual_norm", side, _F16, index)
-            if v.shape != (C,) or not v.is_contiguous():
-                raise KatzError("residual_norm: weight and bias of %s must be contiguous [C] tensors" % side)
-        at.append(v.data_ptr() if v is not None else 0)
-    return norm.code, norm.eps, at[0], at[1]
+def _norm_vector(v, side, C, index):
+    """Address of a norm's weight or bias."""
+    if v is None:
+        return 0
+    if v.dtype is not _F16 or v.get_device() != index or v.dim() != 1 or v.numel() != C or (C > 1 and v.stride(0) != 1):
+        raise KatzError("residual_norm: weight and bias of %s must be contiguous fp16 [C] = [%d] tensors on CUDA device %d (got %s %s on %s)"
+                        % (side, C, index, v.dtype, tuple(v.shape), v.device))
+    return v.data_ptr()
 
 
 def residual_norm(x, y=None, gate=None, post=None, pre=None, scale=None, shift=None, residual_scale=1.0, out=None, normed=None):
@@ -546,7 +551,9 @@ def residual_norm(x, y=None, gate=None, post=None, pre=None, scale=None, shift=N
     dtype = x.dtype
     if dtype is not _F16 and dtype is not _F32:
         raise KatzError("residual_norm: x must be a CUDA fp16 or fp32 tensor (got %s on %s)" % (dtype, x.device))
-    index = _expect(x, "residual_norm", "x", dtype, None)
+    index = x.get_device()
+    if index < 0:
+        _expect(x, "residual_norm", "x", dtype, None)
     shape = x.shape
     if len(shape) == 3:
         B, S, C = shape
@@ -563,17 +570,30 @@ def residual_norm(x, y=None, gate=None, post=None, pre=None, scale=None, shift=N
     if y is None and pre is None:
         raise KatzError("residual_norm: neither y nor pre: nothing to compute")
     x_p = x.data_ptr()
-    x_sb, x_ss = _row_strides(x, "x", shape)
-    y_p = y_sb = y_ss = 0
+    plain = x.is_contiguous()
+    x_sb, x_ss = (S * C, C) if plain else _row_strides(x, "x", shape)
+    y_p = y_sb = y_ss = gate_p = gate_sb = gate_ss = scale_p = scale_sb = scale_ss = shift_p = shift_sb = shift_ss = 0
+    post_kind = post_w = post_b = pre_kind = pre_w = pre_b = 0
+    post_eps = pre_eps = 0.0
+    plain_y = False
     if y is not None:
-        _expect(y, "residual_norm", "y", _F16, index)
-        y_sb, y_ss = _row_strides(y, "y", shape)
+        if y.dtype is not _F16 or y.get_device() != index:
+            _expect(y, "residual_norm", "y", _F16, index)
+        plain_y = y.shape == shape and y.is_contiguous()
+        y_sb, y_ss = (S * C, C) if plain_y else _row_strides(y, "y", shape)
         y_p = y.data_ptr()
-    gate_p, gate_sb, gate_ss = _vector(gate, "gate", shape, index)
-    scale_p, scale_sb, scale_ss = _vector(scale, "scale", shape, index)
-    shift_p, shift_sb, shift_ss = _vector(shift, "shift", shape, index)
-    post_kind, post_eps, post_w, post_b = _norm_vectors(post, "post", C, index)
-    pre_kind, pre_eps, pre_w, pre_b = _norm_vectors(pre, "pre", C, index)
+        if gate is not None:
+            gate_p, gate_sb, gate_ss = _vector(gate, "gate", shape, index)
+        if post is not None:
+            post_kind, post_eps = post.code, post.eps
+            post_w, post_b = _norm_vector(post.weight, "post", C, index), _norm_vector(post.bias, "post", C, index)
+    if pre is not None:
+        pre_kind, pre_eps = pre.code, pre.eps
+        pre_w, pre_b = _norm_vector(pre.weight, "pre", C, index), _norm_vector(pre.bias, "pre", C, index)
+        if scale is not None:
+            scale_p, scale_sb, scale_ss = _vector(scale, "scale", shape, index)
+        if shift is not None:
+            shift_p, shift_sb, shift_ss = _vector(shift, "shift", shape, index)
     h, h_p, h_sb, h_ss = out, 0, S * C, C
     if out is not None:
         _expect(out, "residual_norm", "out", dtype, index)
@@ -584,7 +604,7 @@ def residual_norm(x, y=None, gate=None, post=None, pre=None, scale=None, shift=N
     elif y is None and residual_scale == 1.0:
         h = x
     else:
-        h = x.new_empty(shape)
+        h = torch.empty_like(x) if plain else x.new_empty(shape)      # empty_like is the faster of the two
         h_p = h.data_ptr()
     z, z_p, z_sb, z_ss = normed, 0, S * C, C
     if normed is not None:
@@ -594,7 +614,7 @@ def residual_norm(x, y=None, gate=None, post=None, pre=None, scale=None, shift=N
         if z_p == x_p or z_p == h_p or (z_p == y_p and (z_sb, z_ss) != (y_sb, y_ss)):
             raise KatzError("residual_norm: normed may be y (with the same strides), not x or out")
     elif pre is not None:
-        z = x.new_empty(shape, dtype=_F16)
+        z = torch.empty_like(y) if plain_y else torch.empty_like(x) if plain and dtype is _F16 else x.new_empty(shape, dtype=_F16)
         z_p = z.data_ptr()
     if B and S:
         _call_on(index, "katz_residual_norm_f16", _RESIDUAL_NORM_ARGS.pack(
