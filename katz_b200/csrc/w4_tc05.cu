@@ -8,8 +8,9 @@
 //   * warps 0-11 unpack, in three groups that take turns over units of 128 k: a warp owns 32 weight rows (its TMEM lane
 //     quarter, one row per thread), 64 bytes of codes from shared memory, 64 fp16 pairs to TMEM (tcgen05.st);
 //   * warps 12-15: epilogue, one weight row per thread; for each row of x a warp stores 32 consecutive outputs (64 bytes);
-//   * warp 16: TMA loads of x (128-byte swizzle) into the stages whose A the unpacking warps fill: one barrier says that both
-//     are there; warp 18: TMA loads of codes (64-byte swizzle), a ring of its own so that the HBM stream runs ahead;
+//   * warp 16: TMA loads of x (128-byte swizzle); warp 18: TMA loads of codes (64-byte swizzle); rings of their own, so that
+//     either stream runs ahead of the A stages (with x in the stages of A, of which there are three beside two accumulators
+//     of 160 columns, its latency set the pace);
 //   * warp 19: scales and zero points of 1024 k at a time, gathered into shared memory as fp16 (64 * scale);
 //   * warp 17: tcgen05.mma, D[128 x BT] += A[TMEM] B[x].
 // CTA pairs (PAIR): the MMA covers 256 weight rows, 128 from each CTA's tensor memory, and each CTA loads half of x's tile:
@@ -34,7 +35,7 @@ constexpr int WT_THREADS = 640;
 constexpr int WT_GROUPS = 3, WT_GROUP_WARPS = 4;               // unpacking warps
 constexpr int WT_UNPACK_WARPS = WT_GROUPS * WT_GROUP_WARPS;
 constexpr int WT_EPILOGUE = WT_UNPACK_WARPS, WT_X = WT_EPILOGUE + 4, WT_MMA = WT_X + 1, WT_Q = WT_X + 2;   // first warp of each role
-constexpr int WT_AS = 6, WT_QS = 6, WT_SS = 2;                 // stages of each ring (WT_AS: at most)
+constexpr int WT_XS = 8, WT_AS = 6, WT_QS = 6, WT_SS = 2;      // stages of each ring (x and A: at most)
 // A barrier's parity tells a group that the use before its own is over only if the group knows that the one before THAT is:
 // of A's stages it knows that unit n - WT_GROUPS - stages has been multiplied (its last wait), and must know it of n - 2
 // stages; of the codes' stages it knows the loads of its own units only, n - WT_GROUPS i, and must know that of n - WT_QS.
@@ -43,13 +44,13 @@ constexpr int WT_Q_BYTES = 128 * 64;                           // 128 rows x 128
 constexpr int WT_S_UNITS = 8, WT_S_ROWS = WT_S_UNITS * 128 / 32;      // a scale block: units of 128 k, groups at most
 constexpr int WT_SCALE_BYTES = WT_S_ROWS * 128 * 2, WT_ZERO_BYTES = WT_S_ROWS * 128;
 constexpr int WT_TMEM_COLS = 512;
-constexpr int WT_BARS = 2 * (WT_QS + WT_AS + WT_SS + 2);
+constexpr int WT_BARS = 2 * (WT_XS + WT_QS + WT_AS + WT_SS + 2);
 constexpr int WT_FIXED_SMEM = WT_QS * WT_Q_BYTES + WT_SS * (WT_SCALE_BYTES + WT_ZERO_BYTES) + WT_BARS * 8 + 16 + 1024;
 constexpr int WT_MAX_SMEM = 232448;
 
 struct W4Tile {
     int bt, acc_stride, n_acc;                 // columns of a tile (rows of x), of an accumulator buffer; buffers
-    int stages, x_bytes;              // x_bytes: of x in a stage of this CTA (two boxes of 64 k)
+    int x_stages, x_bytes, a_stages;           // x_bytes: of x in a stage of this CTA (two boxes of 64 k)
     int m_tiles, n_tiles;                      // n_tiles: of 128 rows, of a pair's 256
     bool in_pairs;                             // out (and residual) allow 4-byte accesses to (n, n + 1), n even
     int* status;
@@ -106,22 +107,26 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                                                                        const W4Tile t) {
     extern __shared__ unsigned char smem_raw[];
     const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
-    const uint32_t q_ring = smem + t.stages * t.x_bytes, s_ring = q_ring + WT_QS * WT_Q_BYTES, z_ring = s_ring + WT_SS * WT_SCALE_BYTES,
+    const uint32_t q_ring = smem + t.x_stages * t.x_bytes, s_ring = q_ring + WT_QS * WT_Q_BYTES, z_ring = s_ring + WT_SS * WT_SCALE_BYTES,
                    bars = z_ring + WT_SS * WT_ZERO_BYTES, tmem_slot = bars + WT_BARS * 8;
     const uint32_t q_full = bars, q_empty = q_full + 8 * WT_QS,
                    a_full = q_empty + 8 * WT_QS, a_empty = a_full + 8 * WT_AS, s_full = a_empty + 8 * WT_AS,
-                   s_empty = s_full + 8 * WT_SS, acc_full = s_empty + 8 * WT_SS, acc_empty = acc_full + 16;
+                   s_empty = s_full + 8 * WT_SS, acc_full = s_empty + 8 * WT_SS, acc_empty = acc_full + 16, x_full = acc_empty + 16, x_empty = x_full + 8 * WT_XS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = PAIR ? cluster_ctarank() : 0;
     constexpr int CTAS = PAIR ? 2 : 1;
 
     if (threadIdx.x == 0) {
+        for (int i = 0; i < WT_XS; ++i) {
+            mbar_init(x_full + 8 * i, 1);
+            mbar_init(x_empty + 8 * i, 1);
+        }
         for (int i = 0; i < WT_QS; ++i) {
             mbar_init(q_full + 8 * i, 1);
             mbar_init(q_empty + 8 * i, WT_GROUP_WARPS);
         }
         for (int i = 0; i < WT_AS; ++i) {
-            mbar_init(a_full + 8 * i, WT_GROUP_WARPS * CTAS + 1);      // the unpacking warps and the bytes of x
+            mbar_init(a_full + 8 * i, WT_GROUP_WARPS * CTAS);
             mbar_init(a_empty + 8 * i, 1);
         }
         for (int i = 0; i < WT_SS; ++i) {
@@ -178,7 +183,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
         // of arithmetic.)
         Ring q, a, sc;
         q.skip(group, WT_QS);
-        a.skip(group, t.stages);
+        a.skip(group, t.a_stages);
         const int count = item0 < total ? ((total - 1 - item0) / item_stride + 1) * units : 0;
         int now = 0, mine = group;      // this CTA's units so far; this warp's next one
         bool ok = true;
@@ -207,7 +212,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                     const uint32_t a_bar = 8 * a.s, a_phase = a.phase ^ 1, ta = a_mine + 64 * a.s;
                     mine += WT_GROUPS;
                     q.skip(WT_GROUPS, WT_QS);
-                    a.skip(WT_GROUPS, t.stages);
+                    a.skip(WT_GROUPS, t.a_stages);
                     const bool a_free = mbar_try_wait(a_empty + a_bar, a_phase);
                     const bool q_there = more && mbar_try_wait(q_full + 8 * q.s, q.phase);
                     const uint32_t scales = s_ring + sc.s * WT_SCALE_BYTES + row * 2, zeros = z_ring + sc.s * WT_ZERO_BYTES + row;
@@ -365,31 +370,31 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
     } else if (warp == WT_X) {
         // ---------------------------------------------------------------------------------------- x
         if (elect_one()) {
-            Ring a;
+            Ring x;
             uint32_t issued = 0;
             bool ok = true;
             for (int tile = item0; tile < total && ok; tile += item_stride) {
                 int m0, n0;
                 rows_of(tile, m0, n0);
                 for (int u = 0; u < units; ++u) {
-                    if (!mbar_wait_idle(a_empty + 8 * a.s, a.phase ^ 1)) { ok = false; break; }
-                    const uint32_t dst = smem + a.s * t.x_bytes, half = t.x_bytes / 2;
+                    if (!mbar_wait_idle(x_empty + 8 * x.s, x.phase ^ 1)) { ok = false; break; }
+                    const uint32_t dst = smem + x.s * t.x_bytes, half = t.x_bytes / 2;
                     const bool two = u * 128 + 64 < p.K;      // a tile's last unit may be one box
                     if (PAIR) {
                         // both CTAs' bytes are counted on the leader's barrier, which the leader arms for both
-                        const uint32_t bar = mapa_shared(a_full + 8 * a.s, 0);
+                        const uint32_t bar = mapa_shared(x_full + 8 * x.s, 0);
                         const int m = m0 + (int)rank * (t.bt / 2);
-                        if (rank == 0) mbar_expect_tx(a_full + 8 * a.s, two ? 2 * t.x_bytes : t.x_bytes);
+                        if (rank == 0) mbar_expect_tx(x_full + 8 * x.s, two ? 2 * t.x_bytes : t.x_bytes);
                         tma_load_2d_pair(dst, &tmX, u * 128, m, bar);
                         if (two) tma_load_2d_pair(dst + half, &tmX, u * 128 + 64, m, bar);
                     } else {
-                        const uint32_t bar = a_full + 8 * a.s;
+                        const uint32_t bar = x_full + 8 * x.s;
                         mbar_expect_tx(bar, two ? t.x_bytes : half);
                         tma_load_2d(dst, &tmX, u * 128, m0, bar);
                         if (two) tma_load_2d(dst + half, &tmX, u * 128 + 64, m0, bar);
                     }
                     ++issued;
-                    a.next(t.stages);
+                    x.next(t.x_stages);
                 }
             }
             if (!ok) {
@@ -397,8 +402,8 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                 // copies in flight land before the CTA's shared memory is released (a pair's second CTA waits for the first
                 // in the cluster barrier of the teardown: its copies are counted on the leader's barriers)
                 if (rank == 0) {
-                    const uint32_t n = t.stages, first = issued > n ? issued - n : 0;
-                    for (uint32_t i = first; i < issued; ++i) mbar_wait_idle(a_full + 8 * (i % n), (i / n) & 1);
+                    const uint32_t n = t.x_stages, first = issued > n ? issued - n : 0;
+                    for (uint32_t i = first; i < issued; ++i) mbar_wait_idle(x_full + 8 * (i % n), (i / n) & 1);
                 }
             }
         }
@@ -406,16 +411,16 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
         // ---------------------------------------------------------------------------------------- MMA
         if (rank == 0 && elect_one()) {
             const uint32_t idesc = idesc_f16(PAIR ? 256 : 128, t.bt);
-            Ring a, acc;
+            Ring x, a, acc;
             bool ok = true;
             for (int tile = item0; tile < total && ok; tile += item_stride) {
                 if (!mbar_wait_idle(acc_empty + 8 * acc.s, acc.phase ^ 1)) { ok = false; break; }
                 fence_after_sync();
                 const uint32_t tacc = tmem_base + acc.s * t.acc_stride;
                 for (int u = 0; u < units; ++u) {
-                    if (!mbar_wait_idle(a_full + 8 * a.s, a.phase)) { ok = false; break; }
+                    if (!mbar_wait_idle(a_full + 8 * a.s, a.phase) || !mbar_wait_idle(x_full + 8 * x.s, x.phase)) { ok = false; break; }
                     fence_after_sync();
-                    const uint32_t xs = smem + a.s * t.x_bytes, ta = a_base + 64 * a.s;
+                    const uint32_t xs = smem + x.s * t.x_bytes, ta = a_base + 64 * a.s;
                     auto issue = [&](int b) {      // 64 k
                         const uint64_t bd = smem_desc_sw128(xs + b * (t.x_bytes / 2));
 #pragma unroll
@@ -426,9 +431,15 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                     };
                     issue(0);
                     if (u * 128 + 64 < p.K) issue(1);
-                    if (PAIR) umma_commit_pair(a_empty + 8 * a.s, 3);
-                    else umma_commit(a_empty + 8 * a.s);
-                    a.next(t.stages);
+                    if (PAIR) {
+                        umma_commit_pair(a_empty + 8 * a.s, 3);
+                        umma_commit_pair(x_empty + 8 * x.s, 3);
+                    } else {
+                        umma_commit(a_empty + 8 * a.s);
+                        umma_commit(x_empty + 8 * x.s);
+                    }
+                    a.next(t.a_stages);
+                    x.next(t.x_stages);
                 }
                 if (ok) {
                     if (PAIR) umma_commit_pair(acc_full + 8 * acc.s, 3);
@@ -654,8 +665,9 @@ int linear_w4_tc05(const W4Params& p, cudaStream_t st) {
     t.x_bytes = t.bt * (pair ? 128 : 256);
     const int room = (WT_MAX_SMEM - WT_FIXED_SMEM) / t.x_bytes;
     const int cols = (WT_TMEM_COLS - t.n_acc * t.acc_stride) / 64;
-    t.stages = std::min(std::min(room, cols), WT_AS);
-    KATZ_CHECK_ARG(t.stages >= WT_GROUPS, KATZ_ESIZE);      // holds for every tile the choice above makes
+    t.x_stages = std::min(room, WT_XS);
+    t.a_stages = std::min(cols, WT_AS);
+    KATZ_CHECK_ARG(t.a_stages >= WT_GROUPS && t.x_stages >= 2, KATZ_ESIZE);      // holds for every tile the choice above makes
     t.in_pairs = ((p.N | p.ldo) & 1) == 0 && ((uintptr_t)p.out & 3) == 0 &&
                  (!p.residual || ((p.ldr & 1) == 0 && ((uintptr_t)p.residual & 3) == 0));
     t.status = tc05_status_device_ptr();
@@ -666,7 +678,7 @@ int linear_w4_tc05(const W4Params& p, cudaStream_t st) {
     if (rc) return rc;
     rc = encode_rows(&tq, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_64B, p.q, p.K / 2, p.N, p.K / 2, 64, 128);
     if (rc) return rc;
-    const int smem = t.stages * t.x_bytes + WT_FIXED_SMEM;
+    const int smem = t.x_stages * t.x_bytes + WT_FIXED_SMEM;
     const int tiles = t.m_tiles * t.n_tiles;
     if (pair) launch_k_cluster(linear_w4_tc05_kernel<true>, 2 * (tiles < dev.pairs ? tiles : dev.pairs), WT_THREADS, smem, st, 2, tx, tq, p, t);
     else launch_k_cluster(linear_w4_tc05_kernel<false>, tiles < dev.sms ? tiles : dev.sms, WT_THREADS, smem, st, 1, tx, tq, p, t);
