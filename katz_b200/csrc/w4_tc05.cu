@@ -19,6 +19,7 @@
 // Every mbarrier wait is bounded (tc05.cuh): on a time-out the CTA records a status word, stops storing, frees its TMEM and
 // returns; the host reads the word with katz_tc05_status().
 #include <algorithm>
+#include <type_traits>
 
 #include "tc05.cuh"
 #include "w4.cuh"
@@ -213,8 +214,8 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                     mine += WT_GROUPS;
                     q.skip(WT_GROUPS, WT_QS);
                     a.skip(WT_GROUPS, t.a_stages);
-                    const bool a_free = mbar_try_wait(a_empty + a_bar, a_phase);
-                    const bool q_there = more && mbar_try_wait(q_full + 8 * q.s, q.phase);
+                    const bool a_free = mbar_test(a_empty + a_bar, a_phase);
+                    const bool q_there = more && mbar_test(q_full + 8 * q.s, q.phase);
                     const uint32_t scales = s_ring + sc.s * WT_SCALE_BYTES + row * 2, zeros = z_ring + sc.s * WT_ZERO_BYTES + row;
                     const uint32_t k = (u - u0) * 128;
                     uint32_t w[32];
@@ -282,16 +283,22 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
             // are uniform and each is a loop of its own (as branches per element they took 84 cycles an element).
             const int np = n & ~1, mp = m0 + (lane & 1);
             const uint32_t mine = lane & 1 ? 0x3276u : 0x5410u;
-            auto load_residual = [&](int c, uint32_t* res) {
+            auto load_residual = [&](auto pairs, int c, uint32_t (&res)[8]) {
+                const int left = rows - c;
+                if constexpr (decltype(pairs)::value) {
+                    const __half* src = p.residual + (long long)(mp + c) * p.ldr + np;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    res[i] = 0;
-                    if (t.in_pairs) {
-                        if (in && c + 2 * i + (lane & 1) < rows) res[i] = *reinterpret_cast<const uint32_t*>(p.residual + (long long)(mp + c + 2 * i) * p.ldr + np);
-                    } else if (in) {
-                        const unsigned short* src = reinterpret_cast<const unsigned short*>(p.residual) + (long long)(m0 + c + 2 * i) * p.ldr + n;
-                        if (c + 2 * i < rows) res[i] = src[0];
-                        if (c + 2 * i + 1 < rows) res[i] |= (uint32_t)src[p.ldr] << 16;
+                    for (int i = 0; i < 8; ++i, src += 2 * p.ldr) {
+                        res[i] = 0;
+                        if (in && 2 * i + (lane & 1) < left) res[i] = *reinterpret_cast<const uint32_t*>(src);
+                    }
+                } else {
+                    const unsigned short* src = reinterpret_cast<const unsigned short*>(p.residual) + (long long)(m0 + c) * p.ldr + n;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i, src += 2 * p.ldr) {
+                        res[i] = 0;
+                        if (in && 2 * i < left) res[i] = src[0];
+                        if (in && 2 * i + 1 < left) res[i] |= (uint32_t)src[p.ldr] << 16;
                     }
                 }
             };
@@ -300,64 +307,59 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                 if (n0 + quarter * 32 < p.N)
                     for (int m = lane; m < rows; m += 32, line += 32 * p.ldr) asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
             }
-            uint32_t next_res[2][8];      // the residual of the next two chunks
-            if (p.residual) {
-                load_residual(0, next_res[0]);
-                load_residual(16, next_res[1]);
-            }
-            ok = mbar_wait_idle(acc_full + 8 * acc.s, acc.phase);
-            ok = __all_sync(0xffffffffu, ok);
+            auto store_tile = [&](auto pairs) {
+                constexpr bool PAIRS = decltype(pairs)::value;
+                uint32_t res[8];      // the residual of the next 16 rows of x
+                if (p.residual) load_residual(pairs, 0, res);
+                ok = __all_sync(0xffffffffu, mbar_wait_idle(acc_full + 8 * acc.s, acc.phase));
+                if (!ok) return;
+                fence_after_sync();
+                for (int c = 0; c < rows; c += 16) {
+                    uint32_t r[16];
+                    tmem_ld_32x16(tacc + c, r);
+                    tmem_ld_wait();
+                    float v[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) v[e] = fmaf(__uint_as_float(r[e]), OPERAND_UNSCALE, bias);
+                    if (p.act == KATZ_ACT_SILU) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) v[e] = silu_f(v[e]);
+                    }
+                    if (p.residual) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            uint32_t w = res[i];
+                            if (PAIRS) w = __byte_perm(w, __shfl_xor_sync(0xffffffffu, w, 1), mine);
+                            const float2 f = unpack_half2(w);
+                            v[2 * i] += f.x;
+                            v[2 * i + 1] += f.y;
+                        }
+                        load_residual(pairs, c + 16, res);      // nothing past the last row
+                    }
+                    const int left = rows - c;
+                    uint32_t o[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) o[i] = pack_half2(v[2 * i] * p.out_scale, v[2 * i + 1] * p.out_scale);
+                    if constexpr (PAIRS) {
+                        __half* dst = p.out + (long long)(mp + c) * p.ldo + np;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i, dst += 2 * p.ldo) {
+                            o[i] = __byte_perm(o[i], __shfl_xor_sync(0xffffffffu, o[i], 1), mine);
+                            if (in && 2 * i + (lane & 1) < left) *reinterpret_cast<uint32_t*>(dst) = o[i];
+                        }
+                    } else {
+                        unsigned short* dst = reinterpret_cast<unsigned short*>(p.out) + (long long)(m0 + c) * p.ldo + n;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i, dst += 2 * p.ldo) {
+                            if (in && 2 * i < left) dst[0] = (unsigned short)o[i];
+                            if (in && 2 * i + 1 < left) dst[p.ldo] = (unsigned short)(o[i] >> 16);
+                        }
+                    }
+                }
+            };
+            if (t.in_pairs) store_tile(std::true_type{});
+            else store_tile(std::false_type{});
             if (!ok) break;
-            fence_after_sync();
-            for (int c = 0; c < rows; c += 16) {
-                uint32_t r[16], res[8];
-                tmem_ld_32x16(tacc + c, r);
-                if (p.residual) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        res[i] = next_res[0][i];
-                        next_res[0][i] = next_res[1][i];
-                    }
-                    load_residual(c + 32, next_res[1]);      // nothing past the last row
-                }
-                tmem_ld_wait();
-                float v[16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) v[e] = fmaf(__uint_as_float(r[e]), OPERAND_UNSCALE, bias);
-                if (p.act == KATZ_ACT_SILU) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) v[e] = silu_f(v[e]);
-                }
-                if (p.residual) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        if (t.in_pairs) res[i] = __byte_perm(res[i], __shfl_xor_sync(0xffffffffu, res[i], 1), mine);
-                        const float2 f = unpack_half2(res[i]);
-                        v[2 * i] += f.x;
-                        v[2 * i + 1] += f.y;
-                    }
-                }
-                uint32_t o[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) o[i] = pack_half2(v[2 * i] * p.out_scale, v[2 * i + 1] * p.out_scale);
-                if (t.in_pairs) {
-                    __half* dst = p.out + (long long)(mp + c) * p.ldo + np;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        o[i] = __byte_perm(o[i], __shfl_xor_sync(0xffffffffu, o[i], 1), mine);
-                        if (in && c + 2 * i + (lane & 1) < rows) *reinterpret_cast<uint32_t*>(dst) = o[i];
-                        dst += 2 * p.ldo;
-                    }
-                } else if (in) {
-                    unsigned short* dst = reinterpret_cast<unsigned short*>(p.out) + (long long)(m0 + c) * p.ldo + n;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        if (c + 2 * i < rows) dst[0] = (unsigned short)o[i];
-                        if (c + 2 * i + 1 < rows) dst[p.ldo] = (unsigned short)(o[i] >> 16);
-                        dst += 2 * p.ldo;
-                    }
-                }
-            }
             fence_before_sync();
             __syncwarp();
             if (lane == 0) {
@@ -418,7 +420,9 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                 fence_after_sync();
                 const uint32_t tacc = tmem_base + acc.s * t.acc_stride;
                 for (int u = 0; u < units; ++u) {
-                    if (!mbar_wait_idle(a_full + 8 * a.s, a.phase) || !mbar_wait_idle(x_full + 8 * x.s, x.phase)) { ok = false; break; }
+                    // both barriers are looked at before either is waited for: one round trip where both have been passed
+                    const bool a_there = mbar_test(a_full + 8 * a.s, a.phase), x_there = mbar_test(x_full + 8 * x.s, x.phase);
+                    if (!(a_there && x_there) && !(mbar_wait_idle(a_full + 8 * a.s, a.phase) && mbar_wait_idle(x_full + 8 * x.s, x.phase))) { ok = false; break; }
                     fence_after_sync();
                     const uint32_t xs = smem + x.s * t.x_bytes, ta = a_base + 64 * a.s;
                     auto issue = [&](int b) {      // 64 k
