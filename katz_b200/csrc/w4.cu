@@ -471,9 +471,14 @@ extern "C" int katz_linear_w4_f16(const void* x, long long ldx, const void* q, c
     p.act = act; p.out_scale = out_scale;
     const bool xaligned = aligned16(x) && (M == 1 || ldx % 8 == 0);
     cudaStream_t st = (cudaStream_t)stream;
+    // Few rows go to the kernel of this file while all of x fits shared memory at once: up to 8 rows always (8 x 8192 x 8192:
+    // 20.2 us here, 20.0 us on the tcgen05 path; 8 x 5120 x 1280: 5.8 and 7.9 us; but 8 x 1280 x 10240, where x takes two
+    // turns: 14.0 and 10.8 us), up to 16 for small weights (16 x 1280 x 1280: 4.5 and 7.0 us, 16 x 5120 x 1280: 7.3 and 7.9 us, 16 x
+    // 10240 x 1280: 9.8 and 8.6 us, 16 x 8192 x 8192: 40.7 and 20.0 us). Rows of x that TMA cannot read stay here whatever M.
     RowsLaunch l;
     const bool rows = rows_launch(p, l), tc05 = xaligned && K >= W4_TC05_MIN_K;
-    if (tc05 && (M > 16 || !rows)) return linear_w4_tc05(p, st);
+    const bool few = rows && l.rows >= M && (M <= 8 || (M <= 16 && (long long)N * K <= 8000000));
+    if (tc05 && !few) return linear_w4_tc05(p, st);
     KATZ_CHECK_ARG(rows, KATZ_ESIZE);
     return M <= 8 ? launch_rows<1>(p, l, xaligned, st) : launch_rows<2>(p, l, xaligned, st);
 }

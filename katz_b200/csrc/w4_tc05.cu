@@ -13,6 +13,8 @@
 //     of 160 columns, its latency set the pace);
 //   * warp 19: scales and zero points of 1024 k at a time, gathered into shared memory as fp16 (64 * scale);
 //   * warp 17: tcgen05.mma, D[128 x BT] += A[TMEM] B[x].
+// K split (SPLIT), where there are fewer tiles than SMs: a cluster of 2, 4 or 8 CTAs shares a tile, each multiplies a part of K,
+// and for every 16 rows of x one of them receives the others' sums in its shared memory and adds them in rank order.
 // CTA pairs (PAIR): the MMA covers 256 weight rows, 128 from each CTA's tensor memory, and each CTA loads half of x's tile:
 // per 64 k an SM then fetches BT * 64 + 4096 bytes instead of BT * 128 + 4096, where L2 was the bound.
 //
@@ -53,6 +55,7 @@ struct W4Tile {
     int bt, acc_stride, n_acc;                 // columns of a tile (rows of x), of an accumulator buffer; buffers
     int x_stages, x_bytes, a_stages;           // x_bytes: of x in a stage of this CTA (two boxes of 64 k)
     int m_tiles, n_tiles;                      // n_tiles: of 128 rows, of a pair's 256
+    int split;                                 // CTAs that share a tile (SPLIT)
     bool in_pairs;                             // out (and residual) allow 4-byte accesses to (n, n + 1), n even
     int* status;
 };
@@ -81,6 +84,11 @@ __device__ __forceinline__ uint32_t lds8(uint32_t a) {
     asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
     return v;
 }
+__device__ __forceinline__ float lds_f32(uint32_t a) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
 __device__ __forceinline__ void sts16(uint32_t a, __half v) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"(__half_as_ushort(v)) : "memory"); }
 __device__ __forceinline__ void sts8(uint32_t a, uint32_t v) { asm volatile("st.shared.u8 [%0], %1;" ::"r"(a), "r"(v) : "memory"); }
 
@@ -102,19 +110,21 @@ struct Ring {
     }
 };
 
-template <bool PAIR>
+template <bool PAIR, bool SPLIT>
 __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __grid_constant__ CUtensorMap tmX,
                                                                        const __grid_constant__ CUtensorMap tmQ, const W4Params p,
                                                                        const W4Tile t) {
     extern __shared__ unsigned char smem_raw[];
     const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
     const uint32_t q_ring = smem + t.x_stages * t.x_bytes, s_ring = q_ring + WT_QS * WT_Q_BYTES, z_ring = s_ring + WT_SS * WT_SCALE_BYTES,
-                   bars = z_ring + WT_SS * WT_ZERO_BYTES, tmem_slot = bars + WT_BARS * 8;
+                   bars = z_ring + WT_SS * WT_ZERO_BYTES, tmem_slot = bars + WT_BARS * 8,
+                   sums = tmem_slot + 16;      // SPLIT: [16-row chunk of mine][other rank][16][128] floats
     const uint32_t q_full = bars, q_empty = q_full + 8 * WT_QS,
                    a_full = q_empty + 8 * WT_QS, a_empty = a_full + 8 * WT_AS, s_full = a_empty + 8 * WT_AS,
                    s_empty = s_full + 8 * WT_SS, acc_full = s_empty + 8 * WT_SS, acc_empty = acc_full + 16, x_full = acc_empty + 16, x_empty = x_full + 8 * WT_XS;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = PAIR ? cluster_ctarank() : 0;
+    static_assert(!(PAIR && SPLIT), "a cluster is a pair or a split of K");
+    const uint32_t rank = PAIR ? cluster_ctarank() : 0, part = SPLIT ? cluster_ctarank() : 0;
     constexpr int CTAS = PAIR ? 2 : 1;
 
     if (threadIdx.x == 0) {
@@ -154,14 +164,18 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
     fence_before_sync();
     __syncthreads();
     if (PAIR) cluster_sync_all();      // the peer's barriers are initialised before anything signals them
+    if (SPLIT) cluster_arrive_relaxed();      // this CTA runs; waited for before the first write to another's shared memory
     fence_after_sync();
     uint32_t tmem_base;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot) : "memory");
     const uint32_t a_base = tmem_base + t.n_acc * t.acc_stride;
 
-    const int units = (p.K + 127) >> 7;      // stages of 128 k
+    const int all_units = (p.K + 127) >> 7;      // stages of 128 k; this CTA's: units from first_unit on
+    const int first_unit = SPLIT ? (int)part * all_units / t.split : 0;
+    const int units = SPLIT ? ((int)part + 1) * all_units / t.split - first_unit : all_units;
     const int total = t.m_tiles * t.n_tiles;
-    const int item0 = (int)blockIdx.x / CTAS, item_stride = (int)gridDim.x / CTAS;
+    const int per_item = SPLIT ? t.split : CTAS;
+    const int item0 = (int)blockIdx.x / per_item, item_stride = (int)gridDim.x / per_item;
     auto rows_of = [&](int tile, int& m0, int& n0) {      // weight rows fastest: CTAs at work at one time share x
         const int mt = tile / t.n_tiles;
         m0 = mt * t.bt;
@@ -267,13 +281,33 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
         if (!ok && lane == 0) atomicCAS(t.status, 0, 21);
     } else if (warp < WT_X) {
         // ---------------------------------------------------------------------------------------- epilogue
-        const int quarter = warp & 3;
+        const int quarter = warp & 3, row = quarter * 32 + lane;
         Ring acc;
         bool ok = true;
+        // SPLIT: this CTA's sums of the chunks that other ranks finish go to those; true once every rank has done so
+        auto share_sums = [&](int rows, uint32_t tacc, int row) {
+            const bool done = __all_sync(0xffffffffu, mbar_wait_idle(acc_full, 0));
+            fence_after_sync();
+            cluster_wait();      // the other CTAs run
+            if (done) {
+                for (int i = 0; i * 16 < rows; ++i) {
+                    const uint32_t owner = i % t.split, slot = i / t.split;
+                    if (owner == part) continue;
+                    uint32_t r[16];
+                    tmem_ld_32x16(tacc + 16 * i, r);
+                    tmem_ld_wait();
+                    const uint32_t to = mapa_shared(sums + (slot * (t.split - 1) + part - (part > owner)) * 8192 + row * 4, owner);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + e * 512), "r"(r[e]) : "memory");
+                }
+            }
+            cluster_sync_all();
+            return done;
+        };
         for (int tile = item0; tile < total; tile += item_stride) {
             int m0, n0;
             rows_of(tile, m0, n0);
-            const int n = n0 + quarter * 32 + lane;
+            const int n = n0 + row;
             const bool in = n < p.N;
             const float bias = p.bias && in ? __half2float(p.bias[n]) : 0.f;
             const uint32_t tacc = tmem_base + acc.s * t.acc_stride + ((uint32_t)(quarter * 32) << 16);
@@ -309,16 +343,33 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
             }
             auto store_tile = [&](auto pairs) {
                 constexpr bool PAIRS = decltype(pairs)::value;
+                const int first = SPLIT ? 16 * (int)part : 0, hop = SPLIT ? 16 * t.split : 16;
                 uint32_t res[8];      // the residual of the next 16 rows of x
-                if (p.residual) load_residual(pairs, 0, res);
-                ok = __all_sync(0xffffffffu, mbar_wait_idle(acc_full + 8 * acc.s, acc.phase));
+                if (p.residual) load_residual(pairs, first, res);
+                if constexpr (SPLIT) {
+                    ok = share_sums(rows, tacc, row);
+                } else {
+                    ok = __all_sync(0xffffffffu, mbar_wait_idle(acc_full + 8 * acc.s, acc.phase));
+                    fence_after_sync();
+                }
                 if (!ok) return;
-                fence_after_sync();
-                for (int c = 0; c < rows; c += 16) {
+                for (int c = first; c < rows; c += hop) {
                     uint32_t r[16];
                     tmem_ld_32x16(tacc + c, r);
                     tmem_ld_wait();
                     float v[16];
+                    if constexpr (SPLIT) {
+                        const uint32_t from = sums + (c / hop) * (t.split - 1) * 8192 + row * 4;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) v[e] = 0.f;
+                        for (int s = 0; s < t.split; ++s) {      // in rank order, whichever rank adds
+#pragma unroll
+                            for (int e = 0; e < 16; ++e)
+                                v[e] += s == (int)part ? __uint_as_float(r[e]) : lds_f32(from + (s - (s > (int)part)) * 8192 + e * 512);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(v[e]);
+                    }
 #pragma unroll
                     for (int e = 0; e < 16; ++e) v[e] = fmaf(__uint_as_float(r[e]), OPERAND_UNSCALE, bias);
                     if (p.act == KATZ_ACT_SILU) {
@@ -334,7 +385,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                             v[2 * i] += f.x;
                             v[2 * i + 1] += f.y;
                         }
-                        load_residual(pairs, c + 16, res);      // nothing past the last row
+                        load_residual(pairs, c + hop, res);      // nothing past the last row
                     }
                     const int left = rows - c;
                     uint32_t o[8];
@@ -381,19 +432,20 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                 for (int u = 0; u < units; ++u) {
                     if (!mbar_wait_idle(x_empty + 8 * x.s, x.phase ^ 1)) { ok = false; break; }
                     const uint32_t dst = smem + x.s * t.x_bytes, half = t.x_bytes / 2;
-                    const bool two = u * 128 + 64 < p.K;      // a tile's last unit may be one box
+                    const int k = (first_unit + u) * 128;
+                    const bool two = k + 64 < p.K;      // a tile's last unit may be one box
                     if (PAIR) {
                         // both CTAs' bytes are counted on the leader's barrier, which the leader arms for both
                         const uint32_t bar = mapa_shared(x_full + 8 * x.s, 0);
                         const int m = m0 + (int)rank * (t.bt / 2);
                         if (rank == 0) mbar_expect_tx(x_full + 8 * x.s, two ? 2 * t.x_bytes : t.x_bytes);
-                        tma_load_2d_pair(dst, &tmX, u * 128, m, bar);
-                        if (two) tma_load_2d_pair(dst + half, &tmX, u * 128 + 64, m, bar);
+                        tma_load_2d_pair(dst, &tmX, k, m, bar);
+                        if (two) tma_load_2d_pair(dst + half, &tmX, k + 64, m, bar);
                     } else {
                         const uint32_t bar = x_full + 8 * x.s;
                         mbar_expect_tx(bar, two ? t.x_bytes : half);
-                        tma_load_2d(dst, &tmX, u * 128, m0, bar);
-                        if (two) tma_load_2d(dst + half, &tmX, u * 128 + 64, m0, bar);
+                        tma_load_2d(dst, &tmX, k, m0, bar);
+                        if (two) tma_load_2d(dst + half, &tmX, k + 64, m0, bar);
                     }
                     ++issued;
                     x.next(t.x_stages);
@@ -434,7 +486,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                         }
                     };
                     issue(0);
-                    if (u * 128 + 64 < p.K) issue(1);
+                    if ((first_unit + u) * 128 + 64 < p.K) issue(1);
                     if (PAIR) {
                         umma_commit_pair(a_empty + 8 * a.s, 3);
                         umma_commit_pair(x_empty + 8 * x.s, 3);
@@ -465,7 +517,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                 for (int u = 0; u < units; ++u) {
                     if (!mbar_wait_idle(q_empty + 8 * q.s, q.phase ^ 1)) { ok = false; break; }
                     mbar_expect_tx(q_full + 8 * q.s, WT_Q_BYTES);
-                    tma_load_2d(q_ring + q.s * WT_Q_BYTES, &tmQ, u * 64, n0, q_full + 8 * q.s);
+                    tma_load_2d(q_ring + q.s * WT_Q_BYTES, &tmQ, (first_unit + u) * 64, n0, q_full + 8 * q.s);
                     ++issued;
                     q.next(WT_QS);
                 }
@@ -481,11 +533,12 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
         Ring sc;
         bool ok = true;
         const int per_block = (WT_S_UNITS * 128) >> p.group_shift;
-        const bool by_four = (p.J & 3) == 0 && ((uintptr_t)p.scale & 7) == 0;
+        const bool by_four = ((p.J | (first_unit * 128) >> p.group_shift) & 3) == 0 && ((uintptr_t)p.scale & 7) == 0;
         for (int tile = item0; tile < total && ok; tile += item_stride) {
             int m0, n0;
             rows_of(tile, m0, n0);
-            for (int j0 = 0; j0 < p.J; j0 += per_block) {
+            const int j_end = min(p.J, ((first_unit + units) * 128) >> p.group_shift);
+            for (int j0 = (first_unit * 128) >> p.group_shift; j0 < j_end; j0 += per_block) {
                 ok = mbar_wait_idle(s_empty + 8 * sc.s, sc.phase ^ 1);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
@@ -499,7 +552,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                         for (int u = 0; u < 8; ++u) {
                             const int i = b + u, n = n0 + lane + 32 * (i & 3), jj = i & ~3;
                             v[u] = make_uint2(0, 0);
-                            if (i < per_block && n < p.N && j0 + jj < p.J) v[u] = __ldg(reinterpret_cast<const uint2*>(p.scale + (size_t)n * p.J + j0 + jj));
+                            if (i < per_block && n < p.N && j0 + jj < j_end) v[u] = __ldg(reinterpret_cast<const uint2*>(p.scale + (size_t)n * p.J + j0 + jj));
                         }
 #pragma unroll
                         for (int u = 0; u < 8; ++u) {
@@ -518,7 +571,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
 #pragma unroll
                         for (int u = 0; u < 16; ++u) {
                             const int i = b + u, n = n0 + lane + 32 * (i & 3), jj = i >> 2;
-                            v[u] = n < p.N && j0 + jj < p.J ? __ldg(p.scale + (size_t)n * p.J + j0 + jj) : (unsigned short)0;
+                            v[u] = n < p.N && j0 + jj < j_end ? __ldg(p.scale + (size_t)n * p.J + j0 + jj) : (unsigned short)0;
                         }
 #pragma unroll
                         for (int u = 0; u < 16; ++u) {
@@ -533,7 +586,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
 #pragma unroll
                         for (int u = 0; u < 16; ++u) {
                             const int i = b + u, n = n0 + lane + 32 * (i & 3), jj = i >> 2;
-                            v[u] = n < p.N && j0 + jj < p.J ? __ldg(p.zero + (size_t)n * p.J + j0 + jj) : (unsigned char)0;
+                            v[u] = n < p.N && j0 + jj < j_end ? __ldg(p.zero + (size_t)n * p.J + j0 + jj) : (unsigned char)0;
                         }
 #pragma unroll
                         for (int u = 0; u < 16; ++u) {
@@ -551,6 +604,10 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
     }
     // -------------------------------------------------------------------------------------------- teardown
     __syncwarp();
+    if (SPLIT && (warp < WT_EPILOGUE || warp >= WT_X)) {      // the epilogue warps' two barriers of share_sums()
+        cluster_wait();
+        cluster_sync_all();
+    }
     fence_before_sync();
     __syncthreads();
     if (PAIR) cluster_sync_all();      // neither CTA leaves (or frees TMEM) while the other may still signal it or read its tiles
@@ -592,7 +649,7 @@ static int encode_rows(CUtensorMap* map, CUtensorMapDataType type, CUtensorMapSw
 }
 
 struct W4Device {
-    int sms, pairs;      // CTAs and CTA pairs that are resident at once
+    int slots[4];      // clusters of 1, 2, 4 and 8 CTAs that are resident at once
     bool ready;
 };
 
@@ -600,60 +657,66 @@ static int device_limits(W4Device& out) {
     static W4Device cached[KATZ_MAX_DEVICES] = {};
     W4Device& d = cached[current_device_index()];
     if (!d.ready) {
-        int dev = 0, sms = 0;
+        W4Device found{};
+        int dev = 0;
         cudaError_t e = cudaGetDevice(&dev);
-        if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(linear_w4_tc05_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, WT_MAX_SMEM);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(linear_w4_tc05_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, WT_MAX_SMEM);
+        if (e == cudaSuccess) e = cudaDeviceGetAttribute(&found.slots[0], cudaDevAttrMultiProcessorCount, dev);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(linear_w4_tc05_kernel<false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, WT_MAX_SMEM);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(linear_w4_tc05_kernel<true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, WT_MAX_SMEM);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(linear_w4_tc05_kernel<false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, WT_MAX_SMEM);
+        for (int i = 1; e == cudaSuccess && i < 4; ++i) {
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3((found.slots[0] >> i) << i);
+            cfg.blockDim = dim3(WT_THREADS);
+            cfg.dynamicSmemBytes = WT_MAX_SMEM;
+            cudaLaunchAttribute at[1];
+            at[0].id = cudaLaunchAttributeClusterDimension;
+            at[0].val.clusterDim.x = 1 << i;
+            at[0].val.clusterDim.y = 1;
+            at[0].val.clusterDim.z = 1;
+            cfg.attrs = at;
+            cfg.numAttrs = 1;
+            e = i == 1 ? cudaOccupancyMaxActiveClusters(&found.slots[i], linear_w4_tc05_kernel<true, false>, &cfg)
+                       : cudaOccupancyMaxActiveClusters(&found.slots[i], linear_w4_tc05_kernel<false, true>, &cfg);
+        }
         if (e != cudaSuccess) return (int)e;
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(2 * sms);
-        cfg.blockDim = dim3(WT_THREADS);
-        cfg.dynamicSmemBytes = WT_MAX_SMEM;
-        cudaLaunchAttribute at[1];
-        at[0].id = cudaLaunchAttributeClusterDimension;
-        at[0].val.clusterDim.x = 2;
-        at[0].val.clusterDim.y = 1;
-        at[0].val.clusterDim.z = 1;
-        cfg.attrs = at;
-        cfg.numAttrs = 1;
-        int pairs = 0;
-        e = cudaOccupancyMaxActiveClusters(&pairs, linear_w4_tc05_kernel<true>, &cfg);
-        if (e != cudaSuccess || pairs <= 0) return e != cudaSuccess ? (int)e : KATZ_ENOTREADY;
-        d.sms = sms;
-        d.pairs = pairs;
-        d.ready = true;
+        found.ready = true;
+        d = found;
     }
     out = d;
     return 0;
 }
 
+// bytes of the other ranks' sums that a CTA receives
+static int sums_bytes(int bt, int split) { return (split - 1) * ceil_div(ceil_div(bt, 16), split) * 8192; }
+
 int linear_w4_tc05(const W4Params& p, cudaStream_t st) {
     W4Device dev;
     int rc = device_limits(dev);
     if (rc) return rc;
-    // Tile choice: the least modelled time over the number of tiles along M, alone or in pairs. Per k-step of 64 a CTA
-    // spends 2 BT cycles in the tensor pipe, its loads at about 48 bytes a cycle from L2, and about 190 cycles of unpacking.
-    const int steps = ceil_div(p.K, 64);
+    // Tile choice: the least modelled time (cycles) over the number of tiles along M: single CTAs, pairs, or clusters that
+    // split K. Per unit of 128 k a CTA spends 4 BT cycles in the tensor pipe, its loads at about 48 bytes a cycle from L2, and
+    // 660 cycles of unpacking (measured: 0.35 us a unit for any BT up to 160 alone; 0.47 us for pairs at 160).
+    const int units = ceil_div(p.K, 128);
     W4Tile t{};
     bool pair = false;
     double best = 1e30;
     const int min_tiles = ceil_div(p.M, 256);
     for (int mt = min_tiles; mt <= min_tiles + 8; ++mt) {
-        const int bt = ceil_div(ceil_div(p.M, mt), 16) * 16;
-        const int m_tiles = ceil_div(p.M, bt);
-        for (int two = 0; two < 2; ++two) {
-            if (two && p.N <= 128) continue;
-            const int n_tiles = ceil_div(p.N, two ? 256 : 128), slots = two ? dev.pairs : dev.sms;
+        const int bt = ceil_div(ceil_div(p.M, mt), 16) * 16, m_tiles = ceil_div(p.M, bt);
+        for (int mode = -1; mode < 4; ++mode) {      // -1: pairs; i: K split over 2^i CTAs
+            const bool two = mode < 0;
+            const int split = two ? 1 : 1 << mode, n_tiles = ceil_div(p.N, two ? 256 : 128);
             const long long tiles = (long long)m_tiles * n_tiles;
-            const int n_acc = bt <= 160 && tiles > slots ? 2 : 1;      // three stages of 64 columns beside them
-            const long long waves = ceil_div_ll(tiles, slots);
-            double step = 2.0 * bt, load = (bt * (two ? 64.0 : 128.0) + 4096.0) / 48.0;
-            if (load > step) step = load;
-            if (step < 190.0) step = 190.0;
-            const double drain = 600.0 + 8.0 * bt;
-            const double cost = waves * (steps * step + (n_acc == 1 ? drain : 100.0)) + drain;
-            if (!two && bt > 192) continue;      // two stages of x would be all that fits
+            if (two ? p.N <= 128 : bt > 192) continue;      // a lone CTA has room for two stages of wider x only
+            const int slots = dev.slots[two ? 1 : mode];
+            if (split > 1 && (tiles > slots || units < 2 * split)) continue;
+            const int x_bytes = bt * (two ? 128 : 256);
+            if ((WT_MAX_SMEM - WT_FIXED_SMEM - sums_bytes(bt, split)) / x_bytes < 2) continue;
+            const int n_acc = bt <= 160 && tiles > slots ? 2 : 1;      // three stages of 64 columns beside two accumulators
+            const double waves = (double)ceil_div_ll(tiles, slots), drain = 600.0 + 8.0 * bt;
+            const double unit = std::max(std::max(two ? 5.0 * bt : 4.0 * bt, (x_bytes + 8192.0) / 48.0), 660.0);
+            const double cost = waves * (ceil_div(units, split) * unit + (n_acc == 1 ? drain : 100.0)) + drain + (split > 1 ? 3000.0 : 0.0);
             if (cost < best) {
                 best = cost;
                 pair = two;
@@ -661,16 +724,16 @@ int linear_w4_tc05(const W4Params& p, cudaStream_t st) {
                 t.m_tiles = m_tiles;
                 t.n_tiles = n_tiles;
                 t.n_acc = n_acc;
+                t.split = split;
+                t.x_bytes = x_bytes;
             }
         }
     }
-    KATZ_CHECK_ARG((long long)t.m_tiles * t.n_tiles < (1ll << 30), KATZ_ESIZE);
+    KATZ_CHECK_ARG(best < 1e30 && (long long)t.m_tiles * t.n_tiles < (1ll << 28), KATZ_ESIZE);
     t.acc_stride = ceil_div(t.bt, 32) * 32;
-    t.x_bytes = t.bt * (pair ? 128 : 256);
-    const int room = (WT_MAX_SMEM - WT_FIXED_SMEM) / t.x_bytes;
-    const int cols = (WT_TMEM_COLS - t.n_acc * t.acc_stride) / 64;
-    t.x_stages = std::min(room, WT_XS);
-    t.a_stages = std::min(cols, WT_AS);
+    const int fixed = WT_FIXED_SMEM + sums_bytes(t.bt, t.split);
+    t.x_stages = std::min((WT_MAX_SMEM - fixed) / t.x_bytes, WT_XS);
+    t.a_stages = std::min((WT_TMEM_COLS - t.n_acc * t.acc_stride) / 64, WT_AS);
     KATZ_CHECK_ARG(t.a_stages >= WT_GROUPS && t.x_stages >= 2, KATZ_ESIZE);      // holds for every tile the choice above makes
     t.in_pairs = ((p.N | p.ldo) & 1) == 0 && ((uintptr_t)p.out & 3) == 0 &&
                  (!p.residual || ((p.ldr & 1) == 0 && ((uintptr_t)p.residual & 3) == 0));
@@ -682,10 +745,10 @@ int linear_w4_tc05(const W4Params& p, cudaStream_t st) {
     if (rc) return rc;
     rc = encode_rows(&tq, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_64B, p.q, p.K / 2, p.N, p.K / 2, 64, 128);
     if (rc) return rc;
-    const int smem = t.x_stages * t.x_bytes + WT_FIXED_SMEM;
-    const int tiles = t.m_tiles * t.n_tiles;
-    if (pair) launch_k_cluster(linear_w4_tc05_kernel<true>, 2 * (tiles < dev.pairs ? tiles : dev.pairs), WT_THREADS, smem, st, 2, tx, tq, p, t);
-    else launch_k_cluster(linear_w4_tc05_kernel<false>, tiles < dev.sms ? tiles : dev.sms, WT_THREADS, smem, st, 1, tx, tq, p, t);
+    const int smem = t.x_stages * t.x_bytes + fixed, tiles = t.m_tiles * t.n_tiles;
+    if (t.split > 1) launch_k_cluster(linear_w4_tc05_kernel<false, true>, tiles * t.split, WT_THREADS, smem, st, t.split, tx, tq, p, t);
+    else if (pair) launch_k_cluster(linear_w4_tc05_kernel<true, false>, 2 * std::min(tiles, dev.slots[1]), WT_THREADS, smem, st, 2, tx, tq, p, t);
+    else launch_k_cluster(linear_w4_tc05_kernel<false, false>, std::min(tiles, dev.slots[0]), WT_THREADS, smem, st, 1, tx, tq, p, t);
     KATZ_LAUNCH_RET();
 }
 
