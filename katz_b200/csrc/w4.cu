@@ -147,46 +147,39 @@ static PieceGrid piece_grid(int N, int K, int group, long long ldw) {
 // ---------------------------------------------------------------------------------------------------------------------
 // Few rows: out[M, N] = (act(x W^T + bias) + residual) * out_scale with W in 4 bits.
 //
-// Bound by the stream of codes from HBM and, close behind, by the instructions that turn codes into operands; so scales, x and
-// the loop's bookkeeping are kept out of those.
-// A CTA owns 16 * RT weight rows and up to 8 * MT rows of x; its warps take turns over blocks of 128 k. Lane (g = lane / 4, t =
-// lane % 4) holds the codes of weight rows g and g + 8 as four words of eight k; a word of each row makes the A operands of two
-// m16n8k16 products. The sum over k may be taken in any order as long as both operands use the same one, so the codes are used
-// as they lie in memory, and x is laid out to match once per CTA, in shared memory: the pairs (k, k + 4) that the unpacking
-// gives, 16 bytes a lane and word, no two lanes in one bank. Which k a lane's words cover is chosen by the group size so that
-// the four lanes of a row stay inside ONE group (a lane reads 16, 8 or 4 bytes at a time): a group's products are integers
-// times x, exactly, and its scale multiplies the fp32 sum. CTAs are persistent. Each warp streams its codes through a ring in
-// shared memory with asynchronous copies, across row tiles, every lane reading back what it copied itself: the bytes in
-// flight that HBM needs (some 45 KB an SM) do not fit in registers (one block ahead in registers: 2.8 TB/s). Scales and zero
-// points of a tile lie in shared memory, read row by row while the tile before is multiplied: gathered by the lanes that use
-// them they took more tag lookups than the codes. The warps' sums meet in shared memory, added in warp order.
+// Sixteen weight rows are the M side of m16n8k16 products, up to eight rows of x the N side. Lane (g = lane / 4, t = lane % 4)
+// holds the codes of weight rows g and g + 8 over 32 consecutive k (16 bytes of each, inside one group whatever its size) as
+// four words of eight k; a word of each row makes the A operands of two products. The sum over k may be taken in any order as
+// long as both operands use the same one, so the codes are used as they lie in memory, and x is put into the order that the
+// unpacking gives, pairs (k, k + 4). The warps of a CTA take turns over blocks of 128 k; their sums meet in shared memory, added
+// in warp order. Two kernels differ in how the data reaches the lanes:
+//
+// direct: each lane loads what it needs when it needs it, a CTA for every 16 weight rows. Nothing to set up, but a block's
+// latency stands between two blocks of a warp, and x is fetched again by every CTA. Right for weights whose whole reduction is
+// in flight at once. 1 x 1280 x 1280: 2.3 us (streamed 3.1), 1 x 13760 x 1280: 5.6 us (6.3), 8 x 13760 x 1280: 6.0 us (8.5).
+//
+// stream: persistent CTAs, as many as fit, hold x in shared memory, 16 bytes a lane and word, no two lanes in one bank. Each
+// warp streams its codes through a ring in shared memory with asynchronous copies, across row tiles, every lane reading back
+// what it copied itself: HBM's latency needs some 45 KB in flight an SM. Scales and zero points of a tile lie in shared memory,
+// copied row by row while the tile before is multiplied. 1 x 5120 x 5120: 9.0 us (direct 11.2), 1 x 16384 x 8192 with groups of
+// 128: 20 us (direct 31; the codes alone at HBM's rate: 10), 1 x 32768 x 8192: 36 us (direct 59). What is above HBM's rate
+// is the work a block takes: about 290 cycles of a scheduler, most of them the instructions that turn codes into operands.
+// Where the group is a block (128), the products take the integers code - zero and the scale multiplies their fp32 sum;
+// smaller groups differ from lane to lane, and the scale multiplies the operand (w4.cuh; on the whole block it costs 10% more).
+// (x is rows, N, K here; weights larger than L2, groups of 64 where none are named.)
 constexpr int W4_ROWS_THREADS = 512;
 constexpr int W4_RING = 4;                    // blocks of a warp in flight or in use
 
-// 16, 8 or 4 bytes of codes, global -> shared, zeros if !in. L2 fetches the 256 bytes around them, most of which the CTA's
+// 16 bytes of codes, global -> shared, zeros if !in. L2 fetches the 256 bytes around them, most of which the CTA's
 // other warps are about to ask for: a row at a time a warp reads 64 bytes, and HBM gives such pieces at half its rate.
-template <int BYTES>
 __device__ __forceinline__ void copy_codes(uint32_t dst, const unsigned char* src, bool in) {
-    const int n = in ? BYTES : 0;
-    if (BYTES == 16) asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-    else asm volatile("cp.async.ca.shared.global.L2::256B [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(n), "n"(BYTES) : "memory");
+    asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
 
 // stride of a row of scales in shared memory: an odd number of 4-byte words, so that eight rows lie in different banks
 static __host__ __device__ inline int scale_stride(int J) { return (J + 1) / 2 % 2 ? (J + 1) / 2 * 2 : (J + 1) / 2 * 2 + 2; }
 // bytes of a row of x in shared memory: neighbouring rows 64 bytes apart modulo 128
 static __host__ __device__ inline int x_row_bytes(int K) { return (K + 127) / 128 * 256 + 64; }
-
-// where word i of lane t lies in a block of 128 k, and the reverse for a multiple of eight k
-template <int GROUP>
-struct Words {
-    static constexpr int GROUPS = 128 / GROUP, PER_GROUP = 4 / GROUPS;      // groups a block, words a group
-    static __device__ __forceinline__ int k(int i, int t) { return (i / PER_GROUP) * GROUP + t * (8 * PER_GROUP) + 8 * (i % PER_GROUP); }
-    static __device__ __forceinline__ int slot(int k) {      // 4 i + t
-        const int r = k % GROUP;
-        return 4 * ((k / GROUP) * PER_GROUP + r / 8 % PER_GROUP) + r / (8 * PER_GROUP);
-    }
-};
 
 // eight values of x as the pairs (0,4), (1,5), (2,6), (3,7)
 __device__ __forceinline__ uint4 load_x_pairs(const __half* src, bool aligned) {
@@ -201,154 +194,273 @@ __device__ __forceinline__ uint4 load_x_pairs(const __half* src, bool aligned) {
                       __byte_perm(v.y, v.w, 0x7632));
 }
 
-template <int MT, int GROUP, bool ZERO>
-__global__ void __launch_bounds__(W4_ROWS_THREADS) linear_w4_rows_kernel(const W4Params p, int rows_per_cta, bool xaligned) {
-    typedef Words<GROUP> W;
-    extern __shared__ __align__(16) unsigned char rows_smem[];
-    constexpr int LD = 16 + 4;
-    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int m0 = blockIdx.y * rows_per_cta, rows = min(rows_per_cta, p.M - m0);
-    const int sld = scale_stride(p.J), blocks = (p.K + 127) / 128, xld = x_row_bytes(p.K), tiles = (p.N + 15) / 16;
-    unsigned char* xs = rows_smem;                                                        // [rows][xld]
-    unsigned char* ring = xs + rows_per_cta * xld;                                        // [warp][W4_RING][2 rows][lane][16 bytes]
-    float* red = reinterpret_cast<float*>(ring + warps * W4_RING * 1024);                 // [warp][8 * MT][LD]
-    unsigned short* scales = reinterpret_cast<unsigned short*>(red + warps * 8 * MT * LD);      // [2][16][sld]
-    unsigned char* zeros = reinterpret_cast<unsigned char*>(scales + 2 * 16 * sld);             // [2][16][sld]
-    const uint32_t mine_at = smem_u32(ring) + warp * W4_RING * 1024 + lane * 16;
-    // the next block to copy: of this warp's blocks of tile ctile the one at ck, whose codes of this lane lie at src[]
-    int ctile = blockIdx.x, ck = warp;
-    uint32_t cslot = 0;
-    const unsigned char* src[2];
-    auto at_tile = [&]() {
+// One warp's stream of codes: of row tiles blockIdx.x, + gridDim.x, ... the blocks warp, + warps, ... of 128 k, through W4_RING
+// slots of 1 KB in shared memory. A lane copies, and reads back, its words of weight rows g and g + 8.
+struct CodeStream {
+    const W4Params& p;
+    const int blocks, tiles, warps, warp, g, t;
+    const uint32_t at;      // this lane's place in slot 0
+    int tile, kb;           // the next block to copy
+    uint32_t write_slot = 0, read_slot = 0;
+    const unsigned char* src[2];      // this lane's codes of it
+
+    __device__ __forceinline__ CodeStream(const W4Params& p_, uint32_t ring)
+        : p(p_), blocks((p_.K + 127) / 128), tiles((p_.N + 15) / 16), warps(blockDim.x >> 5), warp(threadIdx.x >> 5),
+          g((threadIdx.x & 31) >> 2), t(threadIdx.x & 3), at(ring + warp * W4_RING * 1024 + (threadIdx.x & 31) * 16), tile(blockIdx.x), kb(warp) {
+        at_tile();
+    }
+    __device__ __forceinline__ void at_tile() {
 #pragma unroll
         for (int h = 0; h < 2; ++h)      // rows past the last are computed and not stored
-            src[h] = p.q + (size_t)min(ctile * 16 + 8 * h + g, p.N - 1) * (p.K / 2) + warp * 64 + 4 * W::PER_GROUP * t;
-    };
-    at_tile();
-    auto copy_next = [&]() {
-        if (ctile < tiles) {
-            // K is a multiple of 32: all of what a lane copies at a time exists, or none (only the last block lacks any)
-            const int left = p.K - ck * 128;
+            src[h] = p.q + (size_t)min(tile * 16 + 8 * h + g, p.N - 1) * (p.K / 2) + warp * 64 + 16 * t;
+    }
+    __device__ __forceinline__ void copy_next() {
+        if (tile < tiles) {
+            // K is a multiple of 32: a lane's codes exist together or not at all (only the last block lacks any)
+            const bool in = kb * 128 + 32 * t < p.K;
 #pragma unroll
-            for (int j = 0; j < W::GROUPS; ++j) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t dst = mine_at + cslot + h * 512 + j * 4 * W::PER_GROUP;
-                    if (left >= 128) copy_codes<4 * W::PER_GROUP>(dst, src[h] + j * (GROUP / 2), true);
-                    else {
-                        const bool in = W::k(j * W::PER_GROUP, t) < left;
-                        copy_codes<4 * W::PER_GROUP>(dst, in ? src[h] + j * (GROUP / 2) : p.q, in);
-                    }
-                }
-            }
-            ck += warps;
+            for (int h = 0; h < 2; ++h) copy_codes(at + write_slot + h * 512, in ? src[h] : p.q, in);
+            kb += warps;
             src[0] += warps * 64;
             src[1] += warps * 64;
-            if (ck >= blocks) {
-                ck = warp;
-                ctile += gridDim.x;
+            if (kb >= blocks) {
+                kb = warp;
+                tile += gridDim.x;
                 at_tile();
             }
         }
         cp_async_commit();
-        cslot = (cslot + 1024) % (W4_RING * 1024);
-    };
-    auto read_scales = [&](int tile, int buf) {
-        for (int r = warp; r < 16; r += warps) {
-            const size_t at = (size_t)min(tile * 16 + r, p.N - 1) * p.J;
-            for (int j = lane; j < p.J; j += 32) {
-                scales[(buf * 16 + r) * sld + j] = __ldg(p.scale + at + j);
-                if (ZERO) zeros[(buf * 16 + r) * sld + j] = __ldg(p.zero + at + j);
+        write_slot = (write_slot + 1024) % (W4_RING * 1024);
+    }
+    __device__ __forceinline__ void start() {
+#pragma unroll
+        for (int i = 0; i < W4_RING - 1; ++i) copy_next();
+    }
+    // the next block's words; requests one more, into the slot that was read in the round before
+    __device__ __forceinline__ void next(uint32_t (&v)[2][4]) {
+        cp_async_wait<W4_RING - 2>();
+        const uint4 a = lds128(at + read_slot), b = lds128(at + read_slot + 512);
+        read_slot = (read_slot + 1024) % (W4_RING * 1024);
+        copy_next();
+        v[0][0] = a.x, v[0][1] = a.y, v[0][2] = a.z, v[0][3] = a.w;
+        v[1][0] = b.x, v[1][1] = b.y, v[1][2] = b.z, v[1][3] = b.w;
+    }
+};
+
+// Scales and zero points of the tiles' rows in shared memory, a buffer of 16 rows a tile. They are copied asynchronously, with
+// the codes of the first block of the tile `ahead` tiles earlier: by that tile's successors' last waits the copy is over
+// (ahead * blocks of a warp >= W4_RING - 1), and the barrier at a tile's end shows it to the other warps. Rows that do not
+// start on 4-byte boundaries (J odd; zero points: J % 4) are loaded and stored.
+struct ScaleRows {
+    int ahead, sld, zld;      // strides of a row of scales (elements) and of zero points (bytes)
+    bool async_scale, async_zero;
+};
+static ScaleRows scale_rows(const W4Params& p, int warps) {
+    ScaleRows s;
+    const int blocks = ceil_div(p.K, 128), least = blocks / warps;      // blocks of the warp that has fewest
+    s.ahead = ceil_div(W4_RING - 1, least > 0 ? least : 1);
+    s.sld = scale_stride(p.J);
+    s.zld = ceil_div(p.J, 4) * 4 + 4;
+    s.async_scale = p.J % 2 == 0 && ((uintptr_t)p.scale & 3) == 0;
+    s.async_zero = p.J % 4 == 0 && ((uintptr_t)p.zero & 3) == 0;
+    return s;
+}
+static long long scale_rows_bytes(const W4Params& p, int warps) {
+    const ScaleRows s = scale_rows(p, warps);
+    return (s.ahead + 1ll) * 16 * (s.sld * 2 + (p.zero ? s.zld : 0));
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+template <bool ZERO>
+__device__ __forceinline__ void read_scales(const W4Params& p, const ScaleRows& s, int tile, unsigned short* scales, unsigned char* zeros) {
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+    for (int r = threadIdx.x >> 5; r < 16; r += warps) {
+        const size_t at = (size_t)min(tile * 16 + r, p.N - 1) * p.J;
+        if (s.async_scale) {
+            for (int j = 2 * lane; j < p.J; j += 64) copy4(smem_u32(scales + r * s.sld + j), p.scale + at + j);
+        } else {
+            for (int j = lane; j < p.J; j += 32) scales[r * s.sld + j] = __ldg(p.scale + at + j);
+        }
+        if (ZERO) {
+            if (s.async_zero) {
+                for (int j = 4 * lane; j < p.J; j += 128) copy4(smem_u32(zeros + r * s.zld + j), p.zero + at + j);
+            } else {
+                for (int j = lane; j < p.J; j += 32) zeros[r * s.zld + j] = __ldg(p.zero + at + j);
             }
         }
-    };
+    }
+}
+
+__device__ __forceinline__ void finish(const W4Params& p, float v, long long m, int n) {
+    if (p.bias) v += __half2float(p.bias[n]);
+    if (p.act == KATZ_ACT_SILU) v = silu_f(v);
+    if (p.residual) v += __half2float(p.residual[m * p.ldr + n]);
+    p.out[m * p.ldo + n] = __float2half_rn(v * p.out_scale);
+}
+
+// Any M (8 * MT rows a CTA) and any alignment of x.
+template <int MT, bool XALIGNED>
+__global__ void __launch_bounds__(W4_ROWS_THREADS) linear_w4_direct_kernel(const __grid_constant__ W4Params p) {
+    __shared__ float red[W4_ROWS_THREADS / 32][8 * MT][16 + 4];
+    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int tiles = (p.N + 15) / 16, n0 = blockIdx.x % tiles * 16, m0 = blockIdx.x / tiles * 8 * MT, blocks = (p.K + 127) / 128;
+    float acc[MT][2][4] = {};      // two chains of products
     pdl_wait();
     pdl_launch_dependents();
+    for (int kb = warp; kb < blocks; kb += warps) {
+        const int k = kb * 128 + 32 * t;
+        const bool in = k < p.K;      // K is a multiple of 32: a lane's 32 k exist together or not at all
+        uint32_t v[2][4];
+        __half2 scale[2], low[2], high[2];
 #pragma unroll
-    for (int i = 0; i < W4_RING - 1; ++i) copy_next();
-    read_scales(blockIdx.x, 0);
-    for (int v = threadIdx.x; v < blocks * 16; v += blockDim.x) {
-        const int k = v * 8;
-        for (int m = 0; m < rows; ++m)
-            *reinterpret_cast<uint4*>(xs + m * xld + (k / 128 * 16 + W::slot(k % 128)) * 16) =
-                k < p.K ? load_x_pairs(p.x + (m0 + m) * p.ldx + k, xaligned) : make_uint4(0, 0, 0, 0);
-    }
-    __syncthreads();
-    // columns of x past the last row hold another row: what they give is not stored
-    const uint32_t x_mine = smem_u32(xs) + 16 * t;
-    uint32_t x_row[MT];
-#pragma unroll
-    for (int c = 0; c < MT; ++c) x_row[c] = x_mine + min(8 * c + g, rows - 1) * xld;
-    uint32_t slot = 0;
-    int buf = 0;
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, buf ^= 1) {
-        if (tile + (int)gridDim.x < tiles) read_scales(tile + gridDim.x, buf ^ 1);      // seen after this tile's barriers
-        const unsigned short* s_row = scales + (buf * 16 + g) * sld;
-        const unsigned char* z_row = zeros + (buf * 16 + g) * sld;
-        float acc[MT][4] = {};
-        for (int kb = warp; kb < blocks; kb += warps) {
-            cp_async_wait<W4_RING - 2>();
-            const uint4 v4[2] = {lds128(mine_at + slot), lds128(mine_at + slot + 512)};
-            slot = (slot + 1024) % (W4_RING * 1024);
-            copy_next();      // into the slot that was read in the round before
-            const uint32_t v[2][4] = {{v4[0].x, v4[0].y, v4[0].z, v4[0].w}, {v4[1].x, v4[1].y, v4[1].z, v4[1].w}};
-#pragma unroll
-            for (int j = 0; j < W::GROUPS; ++j) {
-                float part[MT][2][4];      // two chains of products
-                const int jg = min(kb * W::GROUPS + j, p.J - 1);      // past the last k x is zero
-                __half2 low[2], high[2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    low[h] = as_half2(0xe408e408u);       // -(1024 + 8)
-                    high[h] = as_half2(0xd480d480u);      // -(64 + 8)
-                    if (ZERO) {
-                        const uint32_t z = z_row[8 * h * sld + jg];
-                        low[h] = as_half2(0xe400e400u + z * 0x00010001u);
-                        high[h] = as_half2(0xd400d400u + z * 0x00100010u);
-                    }
-                }
-#pragma unroll
-                for (int i = j * W::PER_GROUP; i < (j + 1) * W::PER_GROUP; ++i) {
-                    __half2 lo[4], hi[4];
-                    unpack8(v[0][i], low[0], high[0], lo);
-                    unpack8(v[1][i], low[1], high[1], hi);
-                    const uint32_t a0[4] = {as_u32(lo[0]), as_u32(hi[0]), as_u32(lo[1]), as_u32(hi[1])};
-                    const uint32_t a1[4] = {as_u32(lo[2]), as_u32(hi[2]), as_u32(lo[3]), as_u32(hi[3])};
-#pragma unroll
-                    for (int c = 0; c < MT; ++c) {
-                        const uint4 b = lds128(x_row[c] + (kb * 4 + i) * 64);
-                        const uint32_t b0[2] = {b.x, b.y}, b1[2] = {b.z, b.w};
-                        if (i % W::PER_GROUP == 0) {
-                            mma_f16_16816_first(part[c][0], a0, b0);
-                            mma_f16_16816_first(part[c][1], a1, b1);
-                        } else {
-                            mma_f16_16816(part[c][0], a0, b0);
-                            mma_f16_16816(part[c][1], a1, b1);
-                        }
-                    }
-                }
-                const float sl = bf16_bits_to_float(s_row[jg]), sh = bf16_bits_to_float(s_row[8 * sld + jg]);
-#pragma unroll
-                for (int c = 0; c < MT; ++c)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[c][e] = fmaf(e < 2 ? sl : sh, part[c][0][e] + part[c][1][e], acc[c][e]);
+        for (int h = 0; h < 2; ++h) {
+            const int n = min(n0 + 8 * h + g, p.N - 1);      // rows past the last are computed and not stored
+            const size_t j = (size_t)n * p.J + (k >> p.group_shift);
+            uint4 w = make_uint4(0, 0, 0, 0);
+            unsigned short sb = 0;
+            uint32_t z = 8;
+            if (in) {
+                w = __ldg(reinterpret_cast<const uint4*>(p.q + (size_t)n * (p.K / 2) + k / 2));
+                sb = __ldg(p.scale + j);
+                if (p.zero) z = __ldg(p.zero + j);
             }
+            v[h][0] = w.x, v[h][1] = w.y, v[h][2] = w.z, v[h][3] = w.w;
+            scale[h] = __float2half2_rn(bf16_bits_to_float(sb) * OPERAND_SCALE);
+            low[h] = as_half2(0xe400e400u + z * 0x00010001u);       // -(1024 + zero)
+            high[h] = as_half2(0xd400d400u + z * 0x00100010u);      // -(64 + zero)
         }
 #pragma unroll
-        for (int c = 0; c < MT; ++c)
+        for (int i = 0; i < 4; ++i) {
+            uint4 b[MT];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) red[(warp * 8 * MT + 8 * c + 2 * t + (e & 1)) * LD + g + 8 * (e >> 1)] = acc[c][e];
+            for (int c = 0; c < MT; ++c) {
+                const int m = m0 + 8 * c + g;
+                b[c] = make_uint4(0, 0, 0, 0);
+                if (in && m < p.M) b[c] = load_x_pairs(p.x + m * p.ldx + k + 8 * i, XALIGNED);
+            }
+            __half2 d[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                unpack8(v[h][i], low[h], high[h], d[h]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) d[h][e] = __hmul2(d[h][e], scale[h]);
+            }
+            const uint32_t a0[4] = {as_u32(d[0][0]), as_u32(d[1][0]), as_u32(d[0][1]), as_u32(d[1][1])};
+            const uint32_t a1[4] = {as_u32(d[0][2]), as_u32(d[1][2]), as_u32(d[0][3]), as_u32(d[1][3])};
+#pragma unroll
+            for (int c = 0; c < MT; ++c) {
+                const uint32_t b0[2] = {b[c].x, b[c].y}, b1[2] = {b[c].z, b[c].w};
+                mma_f16_16816(acc[c][0], a0, b0);
+                mma_f16_16816(acc[c][1], a1, b1);
+            }
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < MT; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) red[warp][8 * c + 2 * t + (e & 1)][g + 8 * (e >> 1)] = acc[c][0][e] + acc[c][1][e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 8 * MT * 16; i += blockDim.x) {
+        const int ml = i / 16, nl = i % 16, n = n0 + nl;
+        const long long m = m0 + ml;
+        if (m >= p.M || n >= p.N) continue;
+        float v = 0.f;
+        for (int w = 0; w < warps; ++w) v += red[w][ml][nl];
+        finish(p, v * OPERAND_UNSCALE, m, n);
+    }
+}
+
+template <bool WIDE, bool ZERO>
+__global__ void __launch_bounds__(W4_ROWS_THREADS) linear_w4_stream_kernel(const __grid_constant__ W4Params p, const ScaleRows sr, bool xaligned) {
+    extern __shared__ __align__(16) unsigned char rows_smem[];
+    constexpr int LD = 16 + 4;
+    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int sld = sr.sld, blocks = (p.K + 127) / 128, xld = x_row_bytes(p.K), tiles = (p.N + 15) / 16;
+    unsigned char* xs = rows_smem;                                                        // [M][xld]
+    unsigned char* ring = xs + p.M * xld;                                                 // [warp][W4_RING][2 rows][lane][16 bytes]
+    float* red = reinterpret_cast<float*>(ring + warps * W4_RING * 1024);                 // [warp][8][LD]
+    unsigned short* scales = reinterpret_cast<unsigned short*>(red + warps * 8 * LD);      // [ahead + 1][16][sld]
+    unsigned char* zeros = reinterpret_cast<unsigned char*>(scales + (sr.ahead + 1) * 16 * sld);      // [ahead + 1][16][zld]
+    CodeStream codes(p, smem_u32(ring));
+    pdl_wait();
+    pdl_launch_dependents();
+    for (int a = 0; a < sr.ahead; ++a)
+        if ((int)blockIdx.x + a * (int)gridDim.x < tiles) read_scales<ZERO>(p, sr, blockIdx.x + a * gridDim.x, scales + a * 16 * sld, zeros + a * 16 * sr.zld);
+    cp_async_commit();
+    codes.start();
+    for (int v = threadIdx.x; v < blocks * 16; v += blockDim.x) {
+        const int k = v * 8;
+        for (int m = 0; m < p.M; ++m)
+            *reinterpret_cast<uint4*>(xs + m * xld + (k / 128 * 16 + k / 8 % 4 * 4 + k / 32 % 4) * 16) =
+                k < p.K ? load_x_pairs(p.x + m * p.ldx + k, xaligned) : make_uint4(0, 0, 0, 0);
+    }
+    cp_async_wait<W4_RING - 1>();      // the first tiles' scales
+    __syncthreads();
+    // columns of x past the last row hold another row: what they give is not stored
+    const uint32_t x_row = smem_u32(xs) + 16 * t + min(g, p.M - 1) * xld;
+    int buf = 0;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, buf = buf == sr.ahead ? 0 : buf + 1) {
+        const long long later = (long long)tile + (long long)sr.ahead * gridDim.x;
+        const int into = buf == 0 ? sr.ahead : buf - 1;      // the buffer that the tile before has left
+        if (later < tiles) read_scales<ZERO>(p, sr, (int)later, scales + into * 16 * sld, zeros + into * 16 * sr.zld);
+        const unsigned short* s_row = scales + (buf * 16 + g) * sld;
+        const unsigned char* z_row = zeros + (buf * 16 + g) * sr.zld;
+        float acc[2][4] = {};      // two chains of products
+        for (int kb = warp; kb < blocks; kb += warps) {
+            uint32_t v[2][4];
+            codes.next(v);
+            const int j = min((kb * 128 + 32 * t) >> p.group_shift, p.J - 1);      // past the last k x is zero
+            __half2 low[2], high[2], scale[2];
+            float wide[2], part[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                low[h] = as_half2(0xe408e408u);       // -(1024 + 8)
+                high[h] = as_half2(0xd480d480u);      // -(64 + 8)
+                if (ZERO) {
+                    const uint32_t z = z_row[8 * h * sr.zld + j];
+                    low[h] = as_half2(0xe400e400u + z * 0x00010001u);
+                    high[h] = as_half2(0xd400d400u + z * 0x00100010u);
+                }
+                wide[h] = bf16_bits_to_float(s_row[8 * h * sld + j]);
+                scale[h] = __float2half2_rn(kb * 128 + 32 * t < p.K ? wide[h] * OPERAND_SCALE : 0.f);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                __half2 d[2][4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    unpack8(v[h][i], low[h], high[h], d[h]);
+                    if (!WIDE)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) d[h][e] = __hmul2(d[h][e], scale[h]);
+                }
+                const uint32_t a0[4] = {as_u32(d[0][0]), as_u32(d[1][0]), as_u32(d[0][1]), as_u32(d[1][1])};
+                const uint32_t a1[4] = {as_u32(d[0][2]), as_u32(d[1][2]), as_u32(d[0][3]), as_u32(d[1][3])};
+                const uint4 b = lds128(x_row + (kb * 4 + i) * 64);
+                const uint32_t b0[2] = {b.x, b.y}, b1[2] = {b.z, b.w};
+                if (WIDE && i == 0) {
+                    mma_f16_16816_first(part[0], a0, b0);
+                    mma_f16_16816_first(part[1], a1, b1);
+                } else {
+                    mma_f16_16816(WIDE ? part[0] : acc[0], a0, b0);
+                    mma_f16_16816(WIDE ? part[1] : acc[1], a1, b1);
+                }
+            }
+            if (WIDE)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[0][e] = fmaf(wide[e >> 1], part[0][e] + part[1][e], acc[0][e]);
+        }
+        cp_async_wait<W4_RING - 2>();      // the next tile's scales (and the next block)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) red[(warp * 8 + 2 * t + (e & 1)) * LD + g + 8 * (e >> 1)] = acc[0][e] + acc[1][e];
         __syncthreads();
-        for (int i = threadIdx.x; i < rows * 16; i += blockDim.x) {
-            const int ml = i / 16, nl = i % 16, n = tile * 16 + nl;
-            const long long m = m0 + ml;
+        for (int i = threadIdx.x; i < p.M * 16; i += blockDim.x) {
+            const int m = i / 16, nl = i % 16, n = tile * 16 + nl;
             if (n >= p.N) continue;
             float v = 0.f;
-            for (int w = 0; w < warps; ++w) v += red[(w * 8 * MT + ml) * LD + nl];
-            if (p.bias) v += __half2float(p.bias[n]);
-            if (p.act == KATZ_ACT_SILU) v = silu_f(v);
-            if (p.residual) v += __half2float(p.residual[m * p.ldr + n]);
-            p.out[m * p.ldo + n] = __float2half_rn(v * p.out_scale);
+            for (int w = 0; w < warps; ++w) v += red[(w * 8 + m) * LD + nl];
+            finish(p, WIDE ? v : v * OPERAND_UNSCALE, m, n);
         }
         __syncthreads();
     }
@@ -365,33 +477,34 @@ static int sm_count() {
     return c;
 }
 
-struct RowsLaunch {
-    int rows, warps;      // of x a CTA
-    size_t smem;
-};
-// false: K is too long for even one row of x and its scales in shared memory
-static bool rows_launch(const W4Params& p, RowsLaunch& l) {
-    const int mt = p.M <= 8 ? 1 : 2, blocks = ceil_div(p.K, 128);
-    for (int most = 8; most <= W4_ROWS_THREADS / 32; most += 8) {
-        // as many warps as share the blocks of k evenly
-        l.warps = ceil_div(blocks, ceil_div(blocks, most));
-        const long long fixed = (long long)l.warps * (W4_RING * 1024 + 8 * mt * 20 * 4) + 2ll * 16 * scale_stride(p.J) * (p.zero ? 3 : 2);
-        const long long fit = (232448 - fixed) / x_row_bytes(p.K);
-        if (fixed >= 232448 || fit < 1) return false;
-        l.rows = (int)std::min<long long>(std::min(p.M, 8 * mt), fit);
-        l.smem = (size_t)(fixed + (long long)l.rows * x_row_bytes(p.K));
-        // Eight warps a CTA where four such CTAs fit an SM: what a tile costs outside its blocks (barriers, sums, scales) is
-        // spread over twice as many of them. With more x in shared memory, or too few tiles to go round, sixteen.
-        if (4 * (l.smem + 1024) <= 233472 && ceil_div(p.N, 16) >= 2 * sm_count()) break;
-    }
-    return true;
+template <int MT>
+static int launch_direct(const W4Params& p, bool xaligned, cudaStream_t st) {
+    const int blocks = ceil_div(p.K, 128);
+    const long long grid = (long long)ceil_div(p.N, 16) * ceil_div(p.M, 8 * MT);
+    KATZ_CHECK_ARG(grid <= 0x7fffffff, KATZ_ESIZE);
+    // as many warps as share the blocks of k evenly: eight, sixteen where the CTAs do not fill the SMs
+    const int most = grid < sm_count() ? 16 : 8, warps = ceil_div(blocks, ceil_div(blocks, most));
+    launch_k(xaligned ? linear_w4_direct_kernel<MT, true> : linear_w4_direct_kernel<MT, false>, (unsigned)grid, warps * 32, 0, st, p);
+    KATZ_LAUNCH_RET();
 }
 
-template <int MT, int GROUP>
-static int launch_rows(const W4Params& p, const RowsLaunch& l, bool xaligned, cudaStream_t st) {
-    const int row_blocks = ceil_div(p.M, l.rows);
-    KATZ_CHECK_ARG(row_blocks <= 65535, KATZ_ESIZE);
-    auto kernel = p.zero ? linear_w4_rows_kernel<MT, GROUP, true> : linear_w4_rows_kernel<MT, GROUP, false>;
+// shared memory of a CTA of the streaming kernel
+static long long stream_smem(const W4Params& p, int warps) {
+    return (long long)p.M * x_row_bytes(p.K) + (long long)warps * (W4_RING * 1024 + 8 * 20 * 4) + scale_rows_bytes(p, warps);
+}
+// Warps of one, as many as share the blocks of k evenly; 0: x and the scales do not fit. Eight where four such CTAs fit an SM:
+// what a tile costs outside its blocks (barriers, sums) is spread over twice as many of them. With more x in shared memory
+// sixteen, if they fit.
+static int stream_warps(const W4Params& p) {
+    const int blocks = ceil_div(p.K, 128), eight = ceil_div(blocks, ceil_div(blocks, 8)), sixteen = ceil_div(blocks, ceil_div(blocks, 16));
+    if (stream_smem(p, eight) > 232448) return 0;
+    return 4 * (stream_smem(p, eight) + 1024) <= 233472 || stream_smem(p, sixteen) > 232448 ? eight : sixteen;
+}
+
+template <bool WIDE>
+static int launch_stream(const W4Params& p, int warps, bool xaligned, cudaStream_t st) {
+    const size_t smem = (size_t)stream_smem(p, warps);
+    auto kernel = p.zero ? linear_w4_stream_kernel<WIDE, true> : linear_w4_stream_kernel<WIDE, false>;
     static bool attr_dev[KATZ_MAX_DEVICES][2] = {};
     bool& attr = attr_dev[current_device_index()][p.zero != nullptr];
     if (!attr) {
@@ -400,18 +513,12 @@ static int launch_rows(const W4Params& p, const RowsLaunch& l, bool xaligned, cu
         attr = true;
     }
     // resident CTAs: 228 KB of shared memory an SM (1 KB of it per CTA), 64 registers a thread
-    const int per_sm = std::max(1, std::min(1024 / (l.warps * 32), (int)(233472 / (l.smem + 1024))));
-    const int slots = std::max(1, sm_count() * per_sm / row_blocks);
-    launch_k(kernel, dim3(std::min(ceil_div(p.N, 16), slots), row_blocks), l.warps * 32, l.smem, st, p, l.rows, xaligned);
+    const int per_sm = std::max(1, std::min(1024 / (warps * 32), (int)(233472 / (smem + 1024))));
+    launch_k(kernel, std::min(ceil_div(p.N, 16), sm_count() * per_sm), warps * 32, smem, st, p, scale_rows(p, warps), xaligned);
     KATZ_LAUNCH_RET();
 }
 
-template <int MT>
-static int launch_rows(const W4Params& p, const RowsLaunch& l, bool xaligned, cudaStream_t st) {
-    if (p.group_shift == 5) return launch_rows<MT, 32>(p, l, xaligned, st);
-    if (p.group_shift == 6) return launch_rows<MT, 64>(p, l, xaligned, st);
-    return launch_rows<MT, 128>(p, l, xaligned, st);
-}
+constexpr int W4_MAX_DIM = 1 << 30;      // indexes of tiles, and a little beyond, stay inside 32 bits
 
 static int group_shift_of(int group) { return group == 32 ? 5 : group == 64 ? 6 : group == 128 ? 7 : -1; }
 
@@ -423,7 +530,7 @@ extern "C" int katz_quantize_w4_f16(const void* w, long long ldw, void* q, void*
     KATZ_CHECK_ARG(w && q && scale, KATZ_EINVAL);
     const int shift = group_shift_of(group);
     KATZ_CHECK_ARG(shift > 0, KATZ_EINVAL);
-    KATZ_CHECK_ARG(N > 0 && K > 0 && K % 32 == 0 && ldw >= K, KATZ_ESIZE);
+    KATZ_CHECK_ARG(N > 0 && K > 0 && K % 32 == 0 && N <= W4_MAX_DIM && K <= W4_MAX_DIM && ldw >= K, KATZ_ESIZE);
     KATZ_CHECK_ARG(aligned16(w) && ldw % 8 == 0 && aligned16(q) && ((uintptr_t)scale & 1) == 0, KATZ_EALIGN);
     const PieceGrid g = piece_grid(N, K, group, ldw);
     KATZ_CHECK_ARG(g.ok, KATZ_ESIZE);
@@ -440,7 +547,7 @@ extern "C" int katz_dequantize_w4_f16(const void* q, const void* scale, const vo
     KATZ_CHECK_ARG(w && q && scale, KATZ_EINVAL);
     const int shift = group_shift_of(group);
     KATZ_CHECK_ARG(shift > 0, KATZ_EINVAL);
-    KATZ_CHECK_ARG(N > 0 && K > 0 && K % 32 == 0 && ldw >= K, KATZ_ESIZE);
+    KATZ_CHECK_ARG(N > 0 && K > 0 && K % 32 == 0 && N <= W4_MAX_DIM && K <= W4_MAX_DIM && ldw >= K, KATZ_ESIZE);
     KATZ_CHECK_ARG(aligned16(w) && ldw % 8 == 0 && aligned16(q) && ((uintptr_t)scale & 1) == 0, KATZ_EALIGN);
     const PieceGrid g = piece_grid(N, K, group, ldw);
     KATZ_CHECK_ARG(g.ok, KATZ_ESIZE);
@@ -459,7 +566,7 @@ extern "C" int katz_linear_w4_f16(const void* x, long long ldx, const void* q, c
     KATZ_CHECK_ARG(act == KATZ_ACT_NONE || act == KATZ_ACT_SILU, KATZ_EINVAL);
     const int shift = group_shift_of(group);
     KATZ_CHECK_ARG(shift > 0, KATZ_EINVAL);
-    KATZ_CHECK_ARG(M > 0 && N > 0 && K > 0 && K % 32 == 0, KATZ_ESIZE);
+    KATZ_CHECK_ARG(M > 0 && N > 0 && K > 0 && K % 32 == 0 && M <= W4_MAX_DIM && N <= W4_MAX_DIM && K <= W4_MAX_DIM, KATZ_ESIZE);
     KATZ_CHECK_ARG((M == 1 || ldx >= K) && (M == 1 || ldo >= N) && (M == 1 || !residual || ldr >= N), KATZ_ESIZE);
     KATZ_CHECK_ARG(aligned16(q) && ((uintptr_t)scale & 1) == 0 && (((uintptr_t)x | (uintptr_t)out | (uintptr_t)bias | (uintptr_t)residual) & 1) == 0,
                    KATZ_EALIGN);
@@ -471,14 +578,16 @@ extern "C" int katz_linear_w4_f16(const void* x, long long ldx, const void* q, c
     p.act = act; p.out_scale = out_scale;
     const bool xaligned = aligned16(x) && (M == 1 || ldx % 8 == 0);
     cudaStream_t st = (cudaStream_t)stream;
-    // Few rows go to the kernel of this file while all of x fits shared memory at once: up to 8 rows always (8 x 8192 x 8192:
-    // 20.2 us here, 20.0 us on the tcgen05 path; 8 x 5120 x 1280: 5.8 and 7.9 us; but 8 x 1280 x 10240, where x takes two
-    // turns: 14.0 and 10.8 us), up to 16 for small weights (16 x 1280 x 1280: 4.5 and 7.0 us, 16 x 5120 x 1280: 7.3 and 7.9 us, 16 x
-    // 10240 x 1280: 9.8 and 8.6 us, 16 x 8192 x 8192: 40.7 and 20.0 us). Rows of x that TMA cannot read stay here whatever M.
-    RowsLaunch l;
-    const bool rows = rows_launch(p, l), tc05 = xaligned && K >= W4_TC05_MIN_K;
-    const bool few = rows && l.rows >= M && (M <= 8 || (M <= 16 && (long long)N * K <= 8000000));
-    if (tc05 && !few) return linear_w4_tc05(p, st);
-    KATZ_CHECK_ARG(rows, KATZ_ESIZE);
-    return M <= 8 ? launch_rows<1>(p, l, xaligned, st) : launch_rows<2>(p, l, xaligned, st);
+    // Up to eight rows: direct while a warp's whole reduction is in flight at once or the weights are few, else streamed (weights
+    // cold, direct / streamed, one row: 1280 x 1280 2.3 / 3.1 us, 40960 x 1280 13.9 / 14.1, 640 x 4096 3.6 / 3.8, 2560 x 2560
+    // 6.2 / 5.0, 1280 x 5120 7.0 / 5.2, 8192 x 10240 21 / 17). Up to sixteen rows: direct while the weights are few, else the
+    // tcgen05 kernel (direct / tcgen05, 16 rows: 1280 x 1280 3.1 / 6.7, 10240 x 1280 7.7 / 8.8, 13760 x 1280 13.4 / 9.2, 1280 x
+    // 5120 9.2 / 9.0, 2560 x 5120 13.5 / 9.9). x that TMA cannot read takes the direct kernel at any size.
+    const bool tc05 = xaligned && K >= W4_TC05_MIN_K;
+    const long long weights = (long long)N * K;
+    const bool streams = M <= 8 && K > 1280 && weights > 3000000;
+    const int warps = streams ? stream_warps(p) : 0;      // 0: too much of x for shared memory
+    if (warps) return shift == 7 ? launch_stream<true>(p, warps, xaligned, st) : launch_stream<false>(p, warps, xaligned, st);
+    if (tc05 && (M > 16 || streams || (M > 8 && weights > (K > 1280 ? 8000000 : 14000000)))) return linear_w4_tc05(p, st);
+    return M <= 8 ? launch_direct<1>(p, xaligned, st) : launch_direct<2>(p, xaligned, st);
 }

@@ -32,9 +32,9 @@ __device__ __forceinline__ uint32_t and_or_1024(uint32_t w) {
     return r;
 }
 
+// One word (8 codes, k = 0..7) -> code - zero as four fp16 pairs (k0,k4), (k1,k5), (k2,k6), (k3,k7):
 //   (word & 0x000f000f) | 0x6400'6400 is the pair (1024 + c0, 1024 + c4) in fp16: subtracting 1024 + zero is exact;
 //   (word & 0x00f000f0) | 0x6400'6400 is (1024 + 16 c1, 1024 + 16 c5): times 1/16, minus 64 + zero, is exact too.
-// One word (8 codes, k = 0..7) -> code - zero as four fp16 pairs (k0,k4), (k1,k5), (k2,k6), (k3,k7)
 __device__ __forceinline__ void unpack8(uint32_t w, __half2 low, __half2 high, __half2* d) {
     const __half2 sixteenth = __float2half2_rn(0.0625f);
     const uint32_t v = w >> 8;

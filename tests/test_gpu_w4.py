@@ -142,6 +142,30 @@ def test_linear_few_rows_of_many_k(cuda_device, M, N, K):
     _linear_case(M, N, K, group=32)
 
 
+# weights that are streamed: odd numbers of groups and rows, short last blocks, and x that leaves shared memory for eight warps
+# but not for sixteen (8 x 10240)
+@pytest.mark.parametrize("M", [1, 3, 8])
+@pytest.mark.parametrize("N,K,group,zeros", [(640, 10240, 64, False), (640, 10240, 64, True), (2403, 1312, 32, True), (1700, 2080, 64, False),
+                                             (2500, 1440, 128, True), (311, 16416, 128, False), (9000, 1376, 32, False)])
+def test_linear_streamed_rows(cuda_device, M, N, K, group, zeros):
+    _linear_case(M, N, K, group=group, zeros=zeros, bias=True, residual=True, silu=M == 3, out_scale=0.5, seed=M + N)
+
+
+@pytest.mark.parametrize("group", [32, 128])
+def test_linear_streamed_rows_of_any_alignment_and_scale(cuda_device, group):
+    from katz_b200 import ops
+    g = _gen(31)
+    N, K = 1700, 2080      # the last block of 128 k is a quarter full
+    q, scale, _ = _weight(g, N, K, group, False)
+    q[:, :] = 0x88      # weights of zero but for one a row ...
+    q[torch.arange(N), torch.arange(N) % (K // 2)] = 0x89
+    scale[:] = 900.0      # ... of 900: code 0 would stand for -7200, outside fp16
+    x = torch.randn(3, K + 9, generator=g, device=cuda_device).half()[:, 1:K + 1]
+    out = ops.linear_w4(x, q, scale, group=group)
+    want = 900.0 * x.double()[:, 2 * (torch.arange(N, device=cuda_device) % (K // 2))]
+    assert torch.allclose(out.double(), want, rtol=2.0 ** -11 + 2.0 ** -23, atol=0)      # one product, one rounding
+
+
 @pytest.mark.parametrize("M", [3, 50, 200])
 def test_linear_strided_unaligned_and_untouched_rows(cuda_device, M):
     """Views with row strides, sources and outputs that start off a 16-byte boundary, `out` = `residual`, and what lies around
