@@ -265,7 +265,7 @@ def quantize_w4(w, group=64, out=None):
     if group not in (32, 64, 128):
         raise KatzError("quantize_w4: group must be 32, 64 or 128 (got %r)" % (group,))
     if out is None:
-        q, scale = w.new_empty((N, K // 2), dtype=_U8), w.new_empty((N, (K + group - 1) // group), dtype=_BF16)
+        q, scale = w.new_empty(N, K // 2, dtype=_U8), w.new_empty(N, (K + group - 1) // group, dtype=_BF16)
     else:
         q, scale = out
         if _w4_check("quantize_w4", q, scale, None, group) != (index, N, K):
@@ -280,7 +280,7 @@ def dequantize_w4(q, scale, zero=None, group=64, out=None):
     index, N, K = _w4_check("dequantize_w4", q, scale, zero, group)
     ld = K
     if out is None:
-        out = q.new_empty((N, K), dtype=_F16)
+        out = q.new_empty(N, K, dtype=_F16)
     else:
         _expect(out, "dequantize_w4", "out", _F16, index)
         ld = _row_stride(out, "dequantize_w4", "out", N, K)
@@ -306,7 +306,7 @@ def linear_w4(x, q, scale, zero=None, group=64, bias=None, residual=None, act=AC
         raise KatzError("linear_w4: unknown activation %r" % (act,))
     ldo = N
     if out is None:
-        out = x.new_empty((M, N))
+        out = x.new_empty(M, N)
     else:
         _expect(out, "linear_w4", "out", _F16, index)
         ldo = _row_stride(out, "linear_w4", "out", M, N)
