@@ -7,7 +7,8 @@
 // persistent CTA per SM, twenty warps:
 //   * warps 0-11 unpack, in three groups that take turns over units of 128 k: a warp owns 32 weight rows (its TMEM lane
 //     quarter, one row per thread), 64 bytes of codes from shared memory, 64 fp16 pairs to TMEM (tcgen05.st);
-//   * warps 12-15: epilogue, one weight row per thread; for each row of x a warp stores 32 consecutive outputs (64 bytes);
+//   * warps 12-15: epilogue, one weight row per thread; for each row of x a warp stores 32 consecutive outputs (64 bytes). At
+//     a CTA's last tile the unpacking warps help;
 //   * warp 16: TMA loads of x (128-byte swizzle); warp 18: TMA loads of codes (64-byte swizzle); rings of their own, so that
 //     either stream runs ahead of the A stages (with x in the stages of A, of which there are three beside two accumulators
 //     of 160 columns, its latency set the pace);
@@ -37,7 +38,7 @@ int* tc05_status_device_ptr();   // defined next to the status word (gemm_tc05.c
 constexpr int WT_THREADS = 640;
 constexpr int WT_GROUPS = 3, WT_GROUP_WARPS = 4;               // unpacking warps
 constexpr int WT_UNPACK_WARPS = WT_GROUPS * WT_GROUP_WARPS;
-constexpr int WT_EPILOGUE = WT_UNPACK_WARPS, WT_X = WT_EPILOGUE + 4, WT_MMA = WT_X + 1, WT_Q = WT_X + 2;   // first warp of each role
+constexpr int WT_EPILOGUE = WT_UNPACK_WARPS, WT_X = WT_EPILOGUE + 4, WT_MMA = WT_X + 1, WT_Q = WT_X + 2, WT_S = WT_X + 3;   // first warp of each role
 constexpr int WT_XS = 8, WT_AS = 6, WT_QS = 6, WT_SS = 2;      // stages of each ring (x and A: at most)
 // A barrier's parity tells a group that the use before its own is over only if the group knows that the one before THAT is:
 // of A's stages it knows that unit n - WT_GROUPS - stages has been multiplied (its last wait), and must know it of n - 2
@@ -47,7 +48,7 @@ constexpr int WT_Q_BYTES = 128 * 64;                           // 128 rows x 128
 constexpr int WT_S_UNITS = 8, WT_S_ROWS = WT_S_UNITS * 128 / 32;      // a scale block: units of 128 k, groups at most
 constexpr int WT_SCALE_BYTES = WT_S_ROWS * 128 * 2, WT_ZERO_BYTES = WT_S_ROWS * 128;
 constexpr int WT_TMEM_COLS = 512;
-constexpr int WT_BARS = 2 * (WT_XS + WT_QS + WT_AS + WT_SS + 2);
+constexpr int WT_BARS = 2 * (WT_XS + WT_QS + WT_AS + WT_SS + 2) + 2;
 constexpr int WT_FIXED_SMEM = WT_QS * WT_Q_BYTES + WT_SS * (WT_SCALE_BYTES + WT_ZERO_BYTES) + WT_BARS * 8 + 16 + 1024;
 constexpr int WT_MAX_SMEM = 232448;
 
@@ -121,7 +122,8 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                    sums = tmem_slot + 16;      // SPLIT: [16-row chunk of mine][other rank][16][128] floats
     const uint32_t q_full = bars, q_empty = q_full + 8 * WT_QS,
                    a_full = q_empty + 8 * WT_QS, a_empty = a_full + 8 * WT_AS, s_full = a_empty + 8 * WT_AS,
-                   s_empty = s_full + 8 * WT_SS, acc_full = s_empty + 8 * WT_SS, acc_empty = acc_full + 16, x_full = acc_empty + 16, x_empty = x_full + 8 * WT_XS;
+                   s_empty = s_full + 8 * WT_SS, acc_full = s_empty + 8 * WT_SS, acc_empty = acc_full + 16, x_full = acc_empty + 16, x_empty = x_full + 8 * WT_XS,
+                   last_full = x_empty + 8 * WT_XS;      // the last tile has a barrier of its own: warps that skipped acc_full cannot tell its parity
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     static_assert(!(PAIR && SPLIT), "a cluster is a pair or a split of K");
     const uint32_t rank = PAIR ? cluster_ctarank() : 0, part = SPLIT ? cluster_ctarank() : 0;
@@ -148,6 +150,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
             mbar_init(acc_full + 8 * i, 1);
             mbar_init(acc_empty + 8 * i, 4 * CTAS);
         }
+        mbar_init(last_full, 1);
         fence_barrier_init();
         tma_prefetch_desc(&tmX);
         tma_prefetch_desc(&tmQ);
@@ -181,11 +184,13 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
         m0 = mt * t.bt;
         n0 = (tile - mt * t.n_tiles) * 128 * CTAS + 128 * (int)rank;
     };
+    const int last = item0 < total ? item0 + (total - 1 - item0) / item_stride * item_stride : -1;      // this CTA's last tile
     // Nothing above touches global memory; every role waits for the kernels this launch depends on before it goes on (those
     // that read none as well: their bounded waits must not run out while a predecessor still runs).
     pdl_wait();
     pdl_launch_dependents();
 
+    bool ok = true;
     if (warp < WT_UNPACK_WARPS) {
         // ---------------------------------------------------------------------------------------- unpack
         const int quarter = warp & 3, group = warp >> 2;
@@ -201,10 +206,9 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
         a.skip(group, t.a_stages);
         const int count = item0 < total ? ((total - 1 - item0) / item_stride + 1) * units : 0;
         int now = 0, mine = group;      // this CTA's units so far; this warp's next one
-        bool ok = true;
         uint4 v0, v1, v2, v3;
-        auto codes = [&](uint32_t c) { return lds128(q_mine + q.s * WT_Q_BYTES + ((c << 4) ^ swz)); };
         auto wait_all = [&](uint32_t bar, uint32_t phase) { return __all_sync(0xffffffffu, mbar_wait(bar, phase)); };
+        auto codes = [&](uint32_t c) { return lds128(q_mine + q.s * WT_Q_BYTES + ((c << 4) ^ swz)); };
         auto free_codes = [&]() {
             __syncwarp();
             if (lane == 0) mbar_arrive(q_empty + 8 * q.s);
@@ -279,147 +283,6 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
             }
         }
         if (!ok && lane == 0) atomicCAS(t.status, 0, 21);
-    } else if (warp < WT_X) {
-        // ---------------------------------------------------------------------------------------- epilogue
-        const int quarter = warp & 3, row = quarter * 32 + lane;
-        Ring acc;
-        bool ok = true;
-        // SPLIT: this CTA's sums of the chunks that other ranks finish go to those; true once every rank has done so
-        auto share_sums = [&](int rows, uint32_t tacc, int row) {
-            const bool done = __all_sync(0xffffffffu, mbar_wait_idle(acc_full, 0));
-            fence_after_sync();
-            cluster_wait();      // the other CTAs run
-            if (done) {
-                for (int i = 0; i * 16 < rows; ++i) {
-                    const uint32_t owner = i % t.split, slot = i / t.split;
-                    if (owner == part) continue;
-                    uint32_t r[16];
-                    tmem_ld_32x16(tacc + 16 * i, r);
-                    tmem_ld_wait();
-                    const uint32_t to = mapa_shared(sums + (slot * (t.split - 1) + part - (part > owner)) * 8192 + row * 4, owner);
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + e * 512), "r"(r[e]) : "memory");
-                }
-            }
-            cluster_sync_all();
-            return done;
-        };
-        for (int tile = item0; tile < total; tile += item_stride) {
-            int m0, n0;
-            rows_of(tile, m0, n0);
-            const int n = n0 + row;
-            const bool in = n < p.N;
-            const float bias = p.bias && in ? __half2float(p.bias[n]) : 0.f;
-            const uint32_t tacc = tmem_base + acc.s * t.acc_stride + ((uint32_t)(quarter * 32) << 16);
-            const int rows = min(t.bt, p.M - m0);
-            // A thread holds one column n of the result and consecutive rows m. Neighbouring threads swap halves so that the
-            // even one has (n, n + 1) of row m and the odd one of row m + 1: a store covers two rows of 64 bytes. The options
-            // are uniform and each is a loop of its own (as branches per element they took 84 cycles an element).
-            const int np = n & ~1, mp = m0 + (lane & 1);
-            const uint32_t mine = lane & 1 ? 0x3276u : 0x5410u;
-            auto load_residual = [&](auto pairs, int c, uint32_t (&res)[8]) {
-                const int left = rows - c;
-                if constexpr (decltype(pairs)::value) {
-                    const __half* src = p.residual + (long long)(mp + c) * p.ldr + np;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i, src += 2 * p.ldr) {
-                        res[i] = 0;
-                        if (in && 2 * i + (lane & 1) < left) res[i] = *reinterpret_cast<const uint32_t*>(src);
-                    }
-                } else {
-                    const unsigned short* src = reinterpret_cast<const unsigned short*>(p.residual) + (long long)(m0 + c) * p.ldr + n;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i, src += 2 * p.ldr) {
-                        res[i] = 0;
-                        if (in && 2 * i < left) res[i] = src[0];
-                        if (in && 2 * i + 1 < left) res[i] |= (uint32_t)src[p.ldr] << 16;
-                    }
-                }
-            };
-            if (p.residual) {      // into L2 while the main loop runs: a lane asks for a row's 64 bytes of this warp
-                const __half* line = p.residual + (long long)(m0 + lane) * p.ldr + n0 + quarter * 32;
-                if (n0 + quarter * 32 < p.N)
-                    for (int m = lane; m < rows; m += 32, line += 32 * p.ldr) asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
-            }
-            auto store_tile = [&](auto pairs) {
-                constexpr bool PAIRS = decltype(pairs)::value;
-                const int first = SPLIT ? 16 * (int)part : 0, hop = SPLIT ? 16 * t.split : 16;
-                uint32_t res[8];      // the residual of the next 16 rows of x
-                if (p.residual) load_residual(pairs, first, res);
-                if constexpr (SPLIT) {
-                    ok = share_sums(rows, tacc, row);
-                } else {
-                    ok = __all_sync(0xffffffffu, mbar_wait_idle(acc_full + 8 * acc.s, acc.phase));
-                    fence_after_sync();
-                }
-                if (!ok) return;
-                for (int c = first; c < rows; c += hop) {
-                    uint32_t r[16];
-                    tmem_ld_32x16(tacc + c, r);
-                    tmem_ld_wait();
-                    float v[16];
-                    if constexpr (SPLIT) {
-                        const uint32_t from = sums + (c / hop) * (t.split - 1) * 8192 + row * 4;
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) v[e] = 0.f;
-                        for (int s = 0; s < t.split; ++s) {      // in rank order, whichever rank adds
-#pragma unroll
-                            for (int e = 0; e < 16; ++e)
-                                v[e] += s == (int)part ? __uint_as_float(r[e]) : lds_f32(from + (s - (s > (int)part)) * 8192 + e * 512);
-                        }
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(v[e]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) v[e] = fmaf(__uint_as_float(r[e]), OPERAND_UNSCALE, bias);
-                    if (p.act == KATZ_ACT_SILU) {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) v[e] = silu_f(v[e]);
-                    }
-                    if (p.residual) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            uint32_t w = res[i];
-                            if (PAIRS) w = __byte_perm(w, __shfl_xor_sync(0xffffffffu, w, 1), mine);
-                            const float2 f = unpack_half2(w);
-                            v[2 * i] += f.x;
-                            v[2 * i + 1] += f.y;
-                        }
-                        load_residual(pairs, c + hop, res);      // nothing past the last row
-                    }
-                    const int left = rows - c;
-                    uint32_t o[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) o[i] = pack_half2(v[2 * i] * p.out_scale, v[2 * i + 1] * p.out_scale);
-                    if constexpr (PAIRS) {
-                        __half* dst = p.out + (long long)(mp + c) * p.ldo + np;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i, dst += 2 * p.ldo) {
-                            o[i] = __byte_perm(o[i], __shfl_xor_sync(0xffffffffu, o[i], 1), mine);
-                            if (in && 2 * i + (lane & 1) < left) *reinterpret_cast<uint32_t*>(dst) = o[i];
-                        }
-                    } else {
-                        unsigned short* dst = reinterpret_cast<unsigned short*>(p.out) + (long long)(m0 + c) * p.ldo + n;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i, dst += 2 * p.ldo) {
-                            if (in && 2 * i < left) dst[0] = (unsigned short)o[i];
-                            if (in && 2 * i + 1 < left) dst[p.ldo] = (unsigned short)(o[i] >> 16);
-                        }
-                    }
-                }
-            };
-            if (t.in_pairs) store_tile(std::true_type{});
-            else store_tile(std::false_type{});
-            if (!ok) break;
-            fence_before_sync();
-            __syncwarp();
-            if (lane == 0) {
-                if (PAIR) mbar_arrive_cluster_tmem(mapa_shared(acc_empty + 8 * acc.s, 0));
-                else mbar_arrive(acc_empty + 8 * acc.s);
-            }
-            acc.next(t.n_acc);
-        }
-        if (!ok && lane == 0) atomicCAS(t.status, 0, 22);
     } else if (warp == WT_X) {
         // ---------------------------------------------------------------------------------------- x
         if (elect_one()) {
@@ -498,8 +361,9 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                     x.next(t.x_stages);
                 }
                 if (ok) {
-                    if (PAIR) umma_commit_pair(acc_full + 8 * acc.s, 3);
-                    else umma_commit(acc_full + 8 * acc.s);
+                    const uint32_t full = tile == last ? last_full : acc_full + 8 * acc.s;
+                    if (PAIR) umma_commit_pair(full, 3);
+                    else umma_commit(full);
                 }
                 acc.next(t.n_acc);
             }
@@ -528,7 +392,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                 for (uint32_t i = first; i < issued; ++i) mbar_wait_idle(q_full + 8 * (i % n), (i / n) & 1);
             }
         }
-    } else {
+    } else if (warp == WT_S) {
         // ---------------------------------------------------------------------------------------- scales, zero points
         Ring sc;
         bool ok = true;
@@ -539,8 +403,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
             rows_of(tile, m0, n0);
             const int j_end = min(p.J, ((first_unit + units) * 128) >> p.group_shift);
             for (int j0 = (first_unit * 128) >> p.group_shift; j0 < j_end; j0 += per_block) {
-                ok = mbar_wait_idle(s_empty + 8 * sc.s, sc.phase ^ 1);
-                ok = __all_sync(0xffffffffu, ok);
+                ok = __all_sync(0xffffffffu, mbar_wait_idle(s_empty + 8 * sc.s, sc.phase ^ 1));
                 if (!ok) break;
                 const uint32_t dst = s_ring + sc.s * WT_SCALE_BYTES + 2 * lane, zdst = z_ring + sc.s * WT_ZERO_BYTES + lane;
                 // groups past the last and rows past the last get zeros: their weights are zeros
@@ -601,6 +464,152 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
             }
         }
         if (!ok && lane == 0) atomicCAS(t.status, 0, 26);
+    }
+    // -------------------------------------------------------------------------------------------- epilogue
+    // Four warps finish the tiles while the others work on the next one. At the last tile nothing is left to unpack, and the
+    // warps that did so share in it: each set of four takes every fourth chunk of 16 rows of x (2048 x 1280 x 5120 with a
+    // residual: 28.6 us without them, 24.7 us with them).
+    if (warp < WT_X && ok && last >= 0 && (!SPLIT || warp >= WT_EPILOGUE)) {
+        // SPLIT: this CTA's sums of the chunks that other ranks finish go to those; true once every rank has done so
+        auto share_sums = [&](int rows, uint32_t tacc, int row) {
+            const bool done = __all_sync(0xffffffffu, mbar_wait_idle(last_full, 0));
+            fence_after_sync();
+            cluster_wait();      // the other CTAs run
+            if (done) {
+                for (int i = 0; i * 16 < rows; ++i) {
+                    const uint32_t owner = i % t.split, slot = i / t.split;
+                    if (owner == part) continue;
+                    uint32_t r[16];
+                    tmem_ld_32x16(tacc + 16 * i, r);
+                    tmem_ld_wait();
+                    const uint32_t to = mapa_shared(sums + (slot * (t.split - 1) + part - (part > owner)) * 8192 + row * 4, owner);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + e * 512), "r"(r[e]) : "memory");
+                }
+            }
+            cluster_sync_all();
+            return done;
+        };
+        Ring acc;
+        if (warp < WT_EPILOGUE) acc.s = (last - item0) / item_stride % t.n_acc;
+        for (int tile = warp < WT_EPILOGUE ? last : item0; tile <= last && ok; tile += item_stride) {
+            const bool shared_tile = tile == last;
+            const int set = shared_tile ? warp >> 2 : 0, sets = shared_tile ? WT_X / 4 : 1;
+            const int quarter = warp & 3, row = quarter * 32 + lane;
+            int m0, n0;
+            rows_of(tile, m0, n0);
+            const int n = n0 + row;
+            const bool in = n < p.N;
+            const float bias = p.bias && in ? __half2float(p.bias[n]) : 0.f;
+            const uint32_t tacc = tmem_base + acc.s * t.acc_stride + ((uint32_t)(quarter * 32) << 16);
+            const int rows = min(t.bt, p.M - m0);
+            // A thread holds one column n of the result and consecutive rows m. Neighbouring threads swap halves so that the
+            // even one has (n, n + 1) of row m and the odd one of row m + 1: a store covers two rows of 64 bytes. The options
+            // are uniform and each is a loop of its own (as branches per element they took 84 cycles an element).
+            const int np = n & ~1, mp = m0 + (lane & 1);
+            const uint32_t mine = lane & 1 ? 0x3276u : 0x5410u;
+            auto load_residual = [&](auto pairs, int c, uint32_t (&res)[8]) {
+                const int left = rows - c;
+                if constexpr (decltype(pairs)::value) {
+                    const __half* src = p.residual + (long long)(mp + c) * p.ldr + np;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i, src += 2 * p.ldr) {
+                        res[i] = 0;
+                        if (in && 2 * i + (lane & 1) < left) res[i] = *reinterpret_cast<const uint32_t*>(src);
+                    }
+                } else {
+                    const unsigned short* src = reinterpret_cast<const unsigned short*>(p.residual) + (long long)(m0 + c) * p.ldr + n;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i, src += 2 * p.ldr) {
+                        res[i] = 0;
+                        if (in && 2 * i < left) res[i] = src[0];
+                        if (in && 2 * i + 1 < left) res[i] |= (uint32_t)src[p.ldr] << 16;
+                    }
+                }
+            };
+            if (p.residual && warp >= WT_EPILOGUE) {      // into L2 while the main loop runs: a lane asks for a row's 64 bytes of this warp
+                const __half* line = p.residual + (long long)(m0 + lane) * p.ldr + n0 + quarter * 32;
+                if (n0 + quarter * 32 < p.N)
+                    for (int m = lane; m < rows; m += 32, line += 32 * p.ldr) asm volatile("prefetch.global.L2 [%0];" ::"l"(line));
+            }
+            auto store_tile = [&](auto pairs) {
+                constexpr bool PAIRS = decltype(pairs)::value;
+                const int first = 16 * (SPLIT ? (int)part : set), hop = 16 * (SPLIT ? t.split : sets);
+                uint32_t res[8];      // the residual of the next 16 rows of x
+                if (p.residual) load_residual(pairs, first, res);
+                if constexpr (SPLIT) {
+                    if (!share_sums(rows, tacc, row)) return false;
+                } else {
+                    if (!__all_sync(0xffffffffu, mbar_wait_idle(shared_tile ? last_full : acc_full + 8 * acc.s, shared_tile ? 0 : acc.phase))) return false;
+                    fence_after_sync();
+                }
+                for (int c = first; c < rows; c += hop) {
+                    uint32_t r[16];
+                    tmem_ld_32x16(tacc + c, r);
+                    tmem_ld_wait();
+                    float v[16];
+                    if constexpr (SPLIT) {
+                        const uint32_t from = sums + (c / hop) * (t.split - 1) * 8192 + row * 4;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) v[e] = 0.f;
+                        for (int s = 0; s < t.split; ++s) {      // in rank order, whichever rank adds
+#pragma unroll
+                            for (int e = 0; e < 16; ++e)
+                                v[e] += s == (int)part ? __uint_as_float(r[e]) : lds_f32(from + (s - (s > (int)part)) * 8192 + e * 512);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(v[e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) v[e] = fmaf(__uint_as_float(r[e]), OPERAND_UNSCALE, bias);
+                    if (p.act == KATZ_ACT_SILU) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) v[e] = silu_f(v[e]);
+                    }
+                    if (p.residual) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            uint32_t w = res[i];
+                            if (PAIRS) w = __byte_perm(w, __shfl_xor_sync(0xffffffffu, w, 1), mine);
+                            const float2 f = unpack_half2(w);
+                            v[2 * i] += f.x;
+                            v[2 * i + 1] += f.y;
+                        }
+                        load_residual(pairs, c + hop, res);      // nothing past the last row
+                    }
+                    const int left = rows - c;
+                    uint32_t o[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) o[i] = pack_half2(v[2 * i] * p.out_scale, v[2 * i + 1] * p.out_scale);
+                    if constexpr (PAIRS) {
+                        __half* dst = p.out + (long long)(mp + c) * p.ldo + np;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i, dst += 2 * p.ldo) {
+                            o[i] = __byte_perm(o[i], __shfl_xor_sync(0xffffffffu, o[i], 1), mine);
+                            if (in && 2 * i + (lane & 1) < left) *reinterpret_cast<uint32_t*>(dst) = o[i];
+                        }
+                    } else {
+                        unsigned short* dst = reinterpret_cast<unsigned short*>(p.out) + (long long)(m0 + c) * p.ldo + n;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i, dst += 2 * p.ldo) {
+                            if (in && 2 * i < left) dst[0] = (unsigned short)o[i];
+                            if (in && 2 * i + 1 < left) dst[p.ldo] = (unsigned short)(o[i] >> 16);
+                        }
+                    }
+                }
+                return true;
+            };
+            ok = t.in_pairs ? store_tile(std::true_type{}) : store_tile(std::false_type{});
+            if (shared_tile || !ok) break;
+            fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+                if (PAIR) mbar_arrive_cluster_tmem(mapa_shared(acc_empty + 8 * acc.s, 0));
+                else mbar_arrive(acc_empty + 8 * acc.s);
+            }
+            acc.next(t.n_acc);
+        }
+        if (!ok && lane == 0) atomicCAS(t.status, 0, 22);
     }
     // -------------------------------------------------------------------------------------------- teardown
     __syncwarp();
