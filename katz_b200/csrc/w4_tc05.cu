@@ -704,8 +704,11 @@ int linear_w4_tc05(const W4Params& p, cudaStream_t st) {
     int rc = device_limits(dev);
     if (rc) return rc;
     // Tile choice: the least modelled time (cycles) over the number of tiles along M: single CTAs, pairs, or clusters that
-    // split K. Per unit of 128 k a CTA spends 4 BT cycles in the tensor pipe, its loads at about 48 bytes a cycle from L2, and
-    // 660 cycles of unpacking (measured: 0.35 us a unit for any BT up to 160 alone; 0.47 us for pairs at 160).
+    // split K. Per unit of 128 k a single CTA spends 4 BT cycles in the tensor pipe, its loads at about 48 bytes a cycle from
+    // L2, and 660 cycles of unpacking (measured: 0.35 us a unit at BT 80, 0.42 at 128, 0.5 at 160); a pair 5.6 BT, at least 820
+    // (0.43 us at 96, 0.5 at 160, 0.6 at 192, 0.75 at 240, all SMs at work and the clock down with them). Between tiles and
+    // after the last one the epilogue, which all warps share at the end. 2048 x 8192 x 8192: pairs of BT 128 218 us, 160 196 us,
+    // 240 189 us, 256 (a last wave half empty) 218 us; 512 x 8192 x 8192: 128 59 us, 256 51 us.
     const int units = ceil_div(p.K, 128);
     W4Tile t{};
     bool pair = false;
@@ -724,8 +727,8 @@ int linear_w4_tc05(const W4Params& p, cudaStream_t st) {
             if ((WT_MAX_SMEM - WT_FIXED_SMEM - sums_bytes(bt, split)) / x_bytes < 2) continue;
             const int n_acc = bt <= 160 && tiles > slots ? 2 : 1;      // three stages of 64 columns beside two accumulators
             const double waves = (double)ceil_div_ll(tiles, slots), drain = 600.0 + 8.0 * bt;
-            const double unit = std::max(std::max(two ? 5.0 * bt : 4.0 * bt, (x_bytes + 8192.0) / 48.0), 660.0);
-            const double cost = waves * (ceil_div(units, split) * unit + (n_acc == 1 ? drain : 100.0)) + drain + (split > 1 ? 3000.0 : 0.0);
+            const double unit = std::max(std::max(two ? 5.6 * bt : 4.0 * bt, (x_bytes + 8192.0) / 48.0), two ? 820.0 : 660.0);
+            const double cost = waves * ceil_div(units, split) * unit + (waves - 1.0) * (n_acc == 1 ? drain : 100.0) + (split > 1 ? drain + 3000.0 : 600.0 + 2.5 * bt);
             if (cost < best) {
                 best = cost;
                 pair = two;
