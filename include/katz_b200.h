@@ -344,10 +344,10 @@ int katz_quantize_w4_f16(const void* w, long long ldw, void* q, void* scale, int
 /* fp16(scale * (code - zero)) -> w [N, K] (row stride ldw, 16-byte aligned rows). */
 int katz_dequantize_w4_f16(const void* q, const void* scale, const void* zero, void* w, long long ldw, int N, int K, int group,
                            void* stream);
-/* out[M, N] = (act(x W^T + bias) + residual) * out_scale with W in 4 bits, fp32 accumulation, any M and N. x, out and
+/* out[M, N] = (act(x W^T + bias) + residual) * out_scale with W in 4 bits, fp32 accumulation, M, N and K up to 2^30. x, out and
  * residual are row-strided (strides in elements, rows do not overlap); residual may be out, x may not. The weight enters the
  * product as an fp16 value of 64 * w: exact for |scale| from 2^-23 to 64 without zero points (with them, code - zero = 9, 11, 13
- * and 15 round in the 12th bit); larger weights than 1023 overflow to infinity. */
+ * and 15 round in the 12th bit); larger weights than 1023 overflow to infinity. x of 16-byte aligned rows is faster. */
 int katz_linear_w4_f16(const void* x, long long ldx, const void* q, const void* scale, const void* zero, int group, void* out,
                        long long ldo, int M, int N, int K, const void* bias, const void* residual, long long ldr, int act,
                        float out_scale, void* stream);

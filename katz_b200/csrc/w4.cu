@@ -19,6 +19,7 @@ using namespace w4;
 // Bound by HBM (2.5 bytes per weight and the scales), which leaves about ten instructions a weight. A lane holds 8 weights; a
 // group is 4, 8 or 16 neighbouring lanes; a warp works on W4_PIECES pieces of 256 weights so that enough loads are in flight.
 // FLAT (contiguous rows of whole groups): the matrix is one run of groups and no lane is idle at a row's end.
+// 166400 x 2048, quantised and read back: 264 us for 1725 MB, HBM's copy rate (6.54 TB/s); 1280 x 1280: 3.7 us, two launches.
 constexpr int W4_PIECES = 4;
 
 __device__ __forceinline__ __half2 hmax2_abs_nan(__half2 a, __half2 b) { return __hmax2_nan(__habs2(a), __habs2(b)); }
@@ -162,8 +163,8 @@ static PieceGrid piece_grid(int N, int K, int group, long long ldw) {
 // warp streams its codes through a ring in shared memory with asynchronous copies, across row tiles, every lane reading back
 // what it copied itself: HBM's latency needs some 45 KB in flight an SM. Scales and zero points of a tile lie in shared memory,
 // copied row by row while the tile before is multiplied. 1 x 5120 x 5120: 9.0 us (direct 11.2), 1 x 16384 x 8192 with groups of
-// 128: 20 us (direct 31; the codes alone at HBM's rate: 10), 1 x 32768 x 8192: 36 us (direct 59). What is above HBM's rate
-// is the work a block takes: about 290 cycles of a scheduler, most of them the instructions that turn codes into operands.
+// 128: 20 us (direct 31; the codes alone at HBM's rate: 10), 1 x 32768 x 8192: 36 us (direct 59). Above HBM's rate it is bound
+// by instructions: some 200 a block and warp (72 turn codes into operands, 8 multiply), the issue slots 64% busy, DRAM 34%.
 // Where the group is a block (128), the products take the integers code - zero and the scale multiplies their fp32 sum;
 // smaller groups differ from lane to lane, and the scale multiplies the operand (w4.cuh; on the whole block it costs 10% more).
 // (x is rows, N, K here; weights larger than L2, groups of 64 where none are named.)

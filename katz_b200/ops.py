@@ -295,8 +295,9 @@ def dequantize_w4(q, scale, zero=None, group=64, out=None):
 def linear_w4(x, q, scale, zero=None, group=64, bias=None, residual=None, act=ACT_NONE, out=None, out_scale=1.0):
     """`linear` with 4-bit weights (the format of quantize_w4, optionally with zero points): out[M,N] = x[M,K] @ w[N,K]^T
     (+bias) -> act -> (+residual) * out_scale, fp32 accumulation, one rounding. Any M (0 included) and N.
-    `x`, `residual`, `out` may be row-strided 2-D views (unit column stride); `out` may be `residual`. Scales of 2^-23 to 64
-    are covered: the weights of larger ones overflow fp16 to infinity, those of smaller ones lose bits."""
+    `x`, `residual`, `out` may be row-strided 2-D views (unit column stride); `out` may be `residual` and overlaps nothing else.
+    Rows of x that do not start on 16-byte boundaries are read by a slower kernel. Scales of 2^-23 to 64 are covered: the
+    weights of larger ones may overflow fp16 to infinity (from 1023 on), those of smaller ones lose bits."""
     index, N, K = _w4_check("linear_w4", q, scale, zero, group)
     if x.dtype is not _F16 or x.get_device() != index:
         _expect(x, "linear_w4", "x", _F16, index)
@@ -547,7 +548,7 @@ def residual_norm(x, y=None, gate=None, post=None, pre=None, scale=None, shift=N
     post, pre: Norm or None. gate, scale, shift: fp16, per channel [C], per sample [B, C], per token [B, S, C] (a 2-D x: [C]
     or [rows, C]); sizes of 1 broadcast and any may be a view into a wider row. h has x's type, z is fp16 and None without
     `pre`; both are rounded once, z from the unrounded h. Without y, h is residual_scale * x (x itself where that is 1 and no
-    `out` is given). `out` (for h) may be x, `normed` (for z) may be y; all last strides are 1."""
+    `out` is given). `out` (for h) may be x, `normed` (for z) may be y, and overlap nothing else; all last strides are 1."""
     dtype = x.dtype
     if dtype is not _F16 and dtype is not _F32:
         raise KatzError("residual_norm: x must be a CUDA fp16 or fp32 tensor (got %s on %s)" % (dtype, x.device))

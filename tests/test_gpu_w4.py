@@ -230,7 +230,7 @@ def test_linear_empty(cuda_device):
     assert ops.dequantize_w4(q[:0], scale[:0]).shape == (0, 256)
 
 
-@pytest.mark.parametrize("M,N,K", [(2, 1280, 1280), (100, 1280, 2048), (500, 640, 2560)])
+@pytest.mark.parametrize("M,N,K", [(2, 1280, 1280), (3, 5120, 2560), (100, 1280, 2048), (500, 640, 2560)])
 def test_linear_repeats_bit_for_bit_on_streams_and_in_graphs(cuda_device, M, N, K):
     from katz_b200 import ops
     g = _gen(8)
