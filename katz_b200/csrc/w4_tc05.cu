@@ -206,6 +206,9 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
         // current one, and polls the two barriers it will need once before the arithmetic, so that a barrier that has long
         // been passed (the usual case) costs nothing. (Waiting where the data was needed, a warp took 1800 cycles for 330
         // of arithmetic.)
+        // A stage of codes goes back to TMA when its unit is in tensor memory, not when its loads have been issued: an arrival does
+        // not wait for shared-memory loads in flight, and where they were delayed TMA's next write overtook them (147 x 3663 x
+        // 7168: in one call of thirty a weight row had the codes of six units later).
         Ring q, a, sc;
         q.skip(group, WT_QS);
         a.skip(group, t.a_stages);
@@ -214,16 +217,9 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
         uint4 v0, v1, v2, v3;
         auto wait_all = [&](uint32_t bar, uint32_t phase) { return __all_sync(0xffffffffu, mbar_wait(bar, phase)); };
         auto codes = [&](uint32_t c) { return lds128(q_mine + q.s * WT_Q_BYTES + ((c << 4) ^ swz)); };
-        auto free_codes = [&]() {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_empty + 8 * q.s);
-        };
         if (mine < count) {
             ok = wait_all(q_full + 8 * q.s, q.phase);
-            if (ok) {
-                v0 = codes(0), v1 = codes(1), v2 = codes(2), v3 = codes(3);
-                free_codes();
-            }
+            if (ok) v0 = codes(0), v1 = codes(1), v2 = codes(2), v3 = codes(3);
         }
         for (int tile = item0; tile < total && ok; tile += item_stride) {
             for (int u0 = 0; u0 < units && ok; u0 += WT_S_UNITS) {
@@ -233,7 +229,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                 const int first = u0 + (mine - now);
                 for (int u = first; u < u1 && ok; u += WT_GROUPS) {
                     const bool more = mine + WT_GROUPS < count;
-                    const uint32_t a_bar = 8 * a.s, a_phase = a.phase ^ 1, ta = a_mine + 64 * a.s;
+                    const uint32_t q_bar = 8 * q.s, a_bar = 8 * a.s, a_phase = a.phase ^ 1, ta = a_mine + 64 * a.s;
                     mine += WT_GROUPS;
                     q.skip(WT_GROUPS, WT_QS);
                     a.skip(WT_GROUPS, t.a_stages);
@@ -272,13 +268,12 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                     if (lane == 0) {
                         if (PAIR) mbar_arrive_cluster_tmem(mapa_shared(a_full + a_bar, 0));      // the leader's MMA thread waits for both CTAs
                         else mbar_arrive(a_full + a_bar);
-                        if (read_now) mbar_arrive(q_empty + 8 * q.s);
+                        mbar_arrive(q_empty + q_bar);
                     }
                     if (more && !read_now) {
                         ok = wait_all(q_full + 8 * q.s, q.phase);
                         if (!ok) break;
                         v0 = codes(0), v1 = codes(1), v2 = codes(2), v3 = codes(3);
-                        free_codes();
                     }
                 }
                 now += u1 - u0;

@@ -267,6 +267,31 @@ def test_linear_repeats_bit_for_bit_on_streams_and_in_graphs(cuda_device, M, N, 
     assert ops.tc05_status() == 0
 
 
+# K split, small groups: the scales arrive later than the codes
+@pytest.mark.parametrize("M,N,K,zeros", [(147, 3663, 7168, False), (300, 5120, 10240, True), (96, 1280, 5120, True)])
+def test_linear_is_the_same_whatever_runs_around_it(cuda_device, M, N, K, zeros):
+    from katz_b200 import ops
+    g = _gen(9)
+    q, scale, zero = _weight(g, N, K, 32, zeros)
+    x = torch.randn(M, K, generator=g, device="cuda").half()
+    r = torch.randn(M, N, generator=g, device="cuda").half()
+    other = torch.randn(1500, 1500, device="cuda")
+    first = ops.linear_w4(x, q, scale, zero=zero, group=32, residual=r)
+    ref.assert_within(first, *ref.linear(x, q, scale, zero, 32, None, r, False, 1.0), "linear_w4")
+    for i in range(20):
+        outs = []
+        for j in range(25):
+            if (i + j) % 3 == 0:
+                other @ other
+            if (i + j) % 5 == 0:
+                torch.cuda._sleep(1000 * (j + 1))
+            if (i + j) % 4 == 0:
+                x + 0
+            outs.append(ops.linear_w4(x, q, scale, zero=zero, group=32, residual=r))
+        assert not any(torch.stack([(o != first).any() for o in outs]).tolist())
+    assert ops.tc05_status() == 0
+
+
 def test_adapter_switch_on_four_bit_weights(cuda_device):
     """The operators as an adapter switch uses them: merge in fp16, remake the 4-bit form in place, multiply; then back."""
     from collections import OrderedDict
