@@ -348,9 +348,21 @@ int katz_dequantize_w4_f16(const void* q, const void* scale, const void* zero, v
  * residual are row-strided (strides in elements, rows do not overlap); residual may be out, x may not. The weight enters the
  * product as an fp16 value of 64 * w: exact for |scale| from 2^-23 to 64 without zero points (with them, code - zero = 9, 11, 13
  * and 15 round in the 12th bit); larger weights than 1023 overflow to infinity. x of 16-byte aligned rows is faster. */
-int katz_linear_w4_f16(const void* x, long long ldx, const void* q, const void* scale, const void* zero, int group, void* out,
-                       long long ldo, int M, int N, int K, const void* bias, const void* residual, long long ldr, int act,
-                       float out_scale, void* stream);
+typedef struct katz_linear_w4_args {
+    const void* x;
+    const void* q;
+    const void* scale;
+    const void* zero;     /* NULL: 8 everywhere */
+    const void* bias;     /* optional [N] */
+    const void* residual; /* optional [M, N] */
+    void* out;
+    long long ldx, ldo, ldr;
+    int M, N, K;
+    int group;
+    int act;
+    float out_scale;
+} katz_linear_w4_args;
+int katz_linear_w4_f16(const katz_linear_w4_args* h_args, void* stream);
 
 /* ------------------------------------------------------------------------------- norms around a gated residual ---- */
 #define KATZ_NORM_NONE 0

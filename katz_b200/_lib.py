@@ -56,6 +56,12 @@ class LinearExtras(Structure):
     _fields_ = [("ln_stats", c_void_p), ("ln_c12", c_void_p), ("ln_slots", c_int), ("ln_eps", c_float), ("stats_out", c_void_p)]
 
 
+class LinearW4Args(Structure):
+    """Mirror of `struct katz_linear_w4_args`."""
+    _fields_ = ([(n, c_void_p) for n in ("x", "q", "scale", "zero", "bias", "residual", "out")] + [(n, c_longlong) for n in ("ldx", "ldo", "ldr")]
+                + [(n, c_int) for n in ("M", "N", "K", "group", "act")] + [("out_scale", c_float)])
+
+
 class ResidualNormArgs(Structure):
     """Mirror of `struct katz_residual_norm_args`."""
     _fields_ = ([(n, c_void_p) for n in ("x", "y", "gate", "scale", "shift", "post_weight", "post_bias", "pre_weight", "pre_bias", "h", "z")]
@@ -130,7 +136,7 @@ SIGNATURES = {
     "katz_euler_cfg_step": (_I, [_V, _V, _V, _L, _F, _F, _F, _I, _V]),
     "katz_quantize_w4_f16": (_I, [_V, _L, _V, _V, _I, _I, _I, _V]),
     "katz_dequantize_w4_f16": (_I, [_V, _V, _V, _V, _L, _I, _I, _I, _V]),
-    "katz_linear_w4_f16": (_I, [_V, _L, _V, _V, _V, _I, _V, _L, _I, _I, _I, _V, _V, _L, _I, _F, _V]),
+    "katz_linear_w4_f16": (_I, [_V, _V]),      # a LinearW4Args, or its bytes
     "katz_residual_norm_f16": (_I, [_V, _V]),      # a ResidualNormArgs, or its bytes
 }
 
@@ -184,6 +190,7 @@ def note_launches(n):
 
 def call(name, *args):
     global _launches
-    lib = load()
-    check(getattr(lib, name)(*args), name)
+    code = getattr(_lib or load(), name)(*args)
+    if code:
+        check(code, name)
     _launches += _KERNELS_PER_CALL.get(name, 1)

@@ -560,24 +560,22 @@ extern "C" int katz_dequantize_w4_f16(const void* q, const void* scale, const vo
     KATZ_LAUNCH_RET();
 }
 
-extern "C" int katz_linear_w4_f16(const void* x, long long ldx, const void* q, const void* scale, const void* zero, int group, void* out,
-                                  long long ldo, int M, int N, int K, const void* bias, const void* residual, long long ldr, int act,
-                                  float out_scale, void* stream) {
-    KATZ_CHECK_ARG(x && q && scale && out, KATZ_EINVAL);
-    KATZ_CHECK_ARG(act == KATZ_ACT_NONE || act == KATZ_ACT_SILU, KATZ_EINVAL);
-    const int shift = group_shift_of(group);
+extern "C" int katz_linear_w4_f16(const katz_linear_w4_args* a, void* stream) {
+    KATZ_CHECK_ARG(a && a->x && a->q && a->scale && a->out, KATZ_EINVAL);
+    KATZ_CHECK_ARG(a->act == KATZ_ACT_NONE || a->act == KATZ_ACT_SILU, KATZ_EINVAL);
+    const int shift = group_shift_of(a->group), M = a->M, N = a->N, K = a->K;
     KATZ_CHECK_ARG(shift > 0, KATZ_EINVAL);
     KATZ_CHECK_ARG(M > 0 && N > 0 && K > 0 && K % 32 == 0 && M <= W4_MAX_DIM && N <= W4_MAX_DIM && K <= W4_MAX_DIM, KATZ_ESIZE);
-    KATZ_CHECK_ARG((M == 1 || ldx >= K) && (M == 1 || ldo >= N) && (M == 1 || !residual || ldr >= N), KATZ_ESIZE);
-    KATZ_CHECK_ARG(aligned16(q) && ((uintptr_t)scale & 1) == 0 && (((uintptr_t)x | (uintptr_t)out | (uintptr_t)bias | (uintptr_t)residual) & 1) == 0,
+    KATZ_CHECK_ARG(M == 1 || (a->ldx >= K && a->ldo >= N && (!a->residual || a->ldr >= N)), KATZ_ESIZE);
+    KATZ_CHECK_ARG(aligned16(a->q) && (((uintptr_t)a->scale | (uintptr_t)a->x | (uintptr_t)a->out | (uintptr_t)a->bias | (uintptr_t)a->residual) & 1) == 0,
                    KATZ_EALIGN);
     W4Params p{};
-    p.x = (const __half*)x; p.q = (const unsigned char*)q; p.scale = (const unsigned short*)scale; p.zero = (const unsigned char*)zero;
-    p.bias = (const __half*)bias; p.residual = (const __half*)residual; p.out = (__half*)out;
-    p.ldx = ldx; p.ldo = ldo; p.ldr = ldr;
-    p.M = M; p.N = N; p.K = K; p.J = ceil_div(K, group); p.group_shift = shift;
-    p.act = act; p.out_scale = out_scale;
-    const bool xaligned = aligned16(x) && (M == 1 || ldx % 8 == 0);
+    p.x = (const __half*)a->x; p.q = (const unsigned char*)a->q; p.scale = (const unsigned short*)a->scale; p.zero = (const unsigned char*)a->zero;
+    p.bias = (const __half*)a->bias; p.residual = (const __half*)a->residual; p.out = (__half*)a->out;
+    p.ldx = a->ldx; p.ldo = a->ldo; p.ldr = a->ldr;
+    p.M = M; p.N = N; p.K = K; p.J = ceil_div(K, a->group); p.group_shift = shift;
+    p.act = a->act; p.out_scale = a->out_scale;
+    const bool xaligned = aligned16(p.x) && (M == 1 || p.ldx % 8 == 0);
     cudaStream_t st = (cudaStream_t)stream;
     // Up to eight rows: direct while a warp's whole reduction is in flight at once or the weights are few, else streamed (weights
     // cold, direct / streamed, one row: 1280 x 1280 2.3 / 3.1 us, 40960 x 1280 13.9 / 14.1, 640 x 4096 3.6 / 3.8, 2560 x 2560

@@ -292,6 +292,11 @@ def dequantize_w4(q, scale, zero=None, group=64, out=None):
     return out
 
 
+# the C records as bytes: packed in 0.2 us, where converting as many arguments one by one takes ctypes 1 us
+_LINEAR_W4_ARGS = struct.Struct("=7Q3q5if")               # katz_linear_w4_args
+_RESIDUAL_NORM_ARGS = struct.Struct("=11Q14q6i3f4x")      # katz_residual_norm_args
+
+
 def linear_w4(x, q, scale, zero=None, group=64, bias=None, residual=None, act=ACT_NONE, out=None, out_scale=1.0):
     """`linear` with 4-bit weights (the format of quantize_w4, optionally with zero points): out[M,N] = x[M,K] @ w[N,K]^T
     (+bias) -> act -> (+residual) * out_scale, fp32 accumulation, one rounding. Any M (0 included) and N.
@@ -313,8 +318,7 @@ def linear_w4(x, q, scale, zero=None, group=64, bias=None, residual=None, act=AC
         ldo = _row_stride(out, "linear_w4", "out", M, N)
         if M and N and out.data_ptr() == x.data_ptr():
             raise KatzError("linear_w4: out must not be x")
-    bias_p = residual_p = None
-    ldr = 0
+    bias_p = residual_p = ldr = 0
     if bias is not None:
         if bias.dtype is not _F16 or bias.get_device() != index:
             _expect(bias, "linear_w4", "bias", _F16, index)
@@ -328,8 +332,9 @@ def linear_w4(x, q, scale, zero=None, group=64, bias=None, residual=None, act=AC
         if ldr != ldo and residual_p == out.data_ptr():
             raise KatzError("linear_w4: residual starts where out does, with another row stride")
     if M and N:
-        _call_on(index, "katz_linear_w4_f16", x.data_ptr(), ldx, q.data_ptr(), scale.data_ptr(), zero.data_ptr() if zero is not None else None,
-                 group, out.data_ptr(), ldo, M, N, K, bias_p, residual_p, ldr, act, out_scale)
+        _call_on(index, "katz_linear_w4_f16", _LINEAR_W4_ARGS.pack(
+            x.data_ptr(), q.data_ptr(), scale.data_ptr(), 0 if zero is None else zero.data_ptr(), bias_p, residual_p, out.data_ptr(),
+            ldx, ldo, ldr, M, N, K, group, act, out_scale))
     return out
 
 
@@ -474,20 +479,27 @@ def layer_norm(x, gamma, beta, eps=1e-5, out=None):
     return out
 
 
+_INF = float("inf")
+
+
 class Norm:
     """A norm of `residual_norm`: kind "layer" ((v - mean) / sqrt(var + eps)) or "rms" (v / sqrt(mean of v^2 + eps)), with optional
     fp16 weight [C] and bias [C]."""
 
+    __slots__ = ("kind", "code", "weight", "bias", "eps")
+    _CODES = {"layer": _lib.NORM_LAYER, "rms": _lib.NORM_RMS}
+
     def __init__(self, kind, weight=None, bias=None, eps=1e-5):
-        if kind not in ("layer", "rms"):
+        code = self._CODES.get(kind)
+        if code is None:
             raise KatzError('Norm: kind must be "layer" or "rms" (got %r)' % (kind,))
-        if not 0.0 <= float(eps) < float("inf"):
+        if not 0.0 <= eps < _INF:
             raise KatzError("Norm: eps must be finite and not negative (got %r)" % (eps,))
-        self.kind, self.weight, self.bias, self.eps = kind, weight, bias, float(eps)
-        self.code = _lib.NORM_LAYER if kind == "layer" else _lib.NORM_RMS
-
-
-_RESIDUAL_NORM_ARGS = struct.Struct("=11Q14q6i3f4x")      # katz_residual_norm_args
+        self.kind = kind
+        self.code = code
+        self.weight = weight
+        self.bias = bias
+        self.eps = eps
 
 
 def _row_strides(t, name, shape):
@@ -512,7 +524,10 @@ def _vector(t, name, shape, index):
     of 1 broadcast."""
     if t.dtype is not _F16 or t.get_device() != index:
         _expect(t, "residual_norm", name, _F16, index)
-    ts, st = t.shape, t.stride()
+    ts = t.shape
+    if len(ts) == 1 and ts[0] == shape[-1] and t.is_contiguous():
+        return t.data_ptr(), 0, 0
+    st = t.stride()
     d, full = len(ts), len(shape)
     ok = 0 < d <= full and ts[-1] == shape[-1] and (st[-1] == 1 or ts[-1] == 1)
     sb = ss = 0
@@ -535,7 +550,7 @@ def _norm_vector(v, side, C, index):
     """Address of a norm's weight or bias."""
     if v is None:
         return 0
-    if v.dtype is not _F16 or v.get_device() != index or v.dim() != 1 or v.numel() != C or (C > 1 and v.stride(0) != 1):
+    if v.dtype is not _F16 or v.get_device() != index or v.shape != (C,) or not v.is_contiguous():
         raise KatzError("residual_norm: weight and bias of %s must be contiguous fp16 [C] = [%d] tensors on CUDA device %d (got %s %s on %s)"
                         % (side, C, index, v.dtype, tuple(v.shape), v.device))
     return v.data_ptr()

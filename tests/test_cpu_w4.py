@@ -22,7 +22,10 @@ def test_entry_points_refuse_bad_arguments_without_a_device():
         assert f(w=P + 2) == f(q=P + 8) == f(s=P + 1) == f(ldw=260) == -2
 
     def lin(x=P, ldx=256, q=P, s=P, z=None, g=64, o=P, ldo=8, M=4, N=8, K=256, b=None, r=None, ldr=0, act=0):
-        return lib.katz_linear_w4_f16(x, ldx, q, s, z, g, o, ldo, M, N, K, b, r, ldr, act, 1.0, None)
+        a = _lib.LinearW4Args(x=x, q=q, scale=s, zero=z, bias=b, residual=r, out=o, ldx=ldx, ldo=ldo, ldr=ldr, M=M, N=N, K=K, group=g, act=act,
+                              out_scale=1.0)
+        return lib.katz_linear_w4_f16(ctypes.byref(a), None)
+    assert lib.katz_linear_w4_f16(None, None) == -1
     assert lin(x=None) == lin(q=None) == lin(s=None) == lin(o=None) == lin(act=2) == lin(act=-1) == lin(g=33) == -1
     assert lin(M=0) == lin(N=0) == lin(K=0) == lin(K=250) == lin(M=-1) == lin(ldx=255) == lin(ldo=7) == lin(r=P, ldr=7) == -3
     assert lin(q=P + 1) == lin(s=P + 1) == lin(x=P + 1) == lin(o=P + 1) == lin(b=P + 1) == lin(r=P + 1, ldr=8) == -2
@@ -47,6 +50,9 @@ def test_residual_norm_refuses_bad_arguments_without_a_device():
 def test_struct_mirrors_the_header():
     from katz_b200 import _lib, ops
     assert ctypes.sizeof(_lib.ResidualNormArgs) == 11 * 8 + 14 * 8 + 6 * 4 + 3 * 4 + 4      # padded to 8
+    assert ctypes.sizeof(_lib.LinearW4Args) == 7 * 8 + 3 * 8 + 5 * 4 + 4
+    a = _lib.LinearW4Args.from_buffer_copy(ops._LINEAR_W4_ARGS.pack(*range(1, 16), 0.25))
+    assert [getattr(a, n) for n, _ in a._fields_] == list(range(1, 16)) + [0.25]
     # the packed form that the wrapper passes is the same record
     packed = ops._RESIDUAL_NORM_ARGS.pack(*range(1, 32), 0.25, 0.5, 0.75)
     a = _lib.ResidualNormArgs.from_buffer_copy(packed)
