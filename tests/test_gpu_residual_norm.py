@@ -168,6 +168,20 @@ def test_streams_graphs_and_repeats(cuda_device):
     assert torch.equal(hg, h3) and torch.equal(zg, z3)
 
 
+def test_more_than_four_gigabytes(cuda_device):
+    from katz_b200 import ops
+    B, S, C = 3, 600000, 1280      # 2.3e9 elements
+    x = torch.zeros(B, S, C, device="cuda", dtype=torch.float16)
+    g = _gen(5)
+    x[:, -3:] = torch.randn(B, 3, C, generator=g, device="cuda").half()
+    scale = _vector(g, "sample", B, S, C)
+    h, z = ops.residual_norm(x, x, pre=ops.Norm("rms"), scale=scale, residual_scale=0.5)
+    first, second = ref.residual_norm(x[:, -3:], x[:, -3:], None, None, ("rms", None, None, 1e-5), scale, None, 0.5)
+    ref.assert_within(h[:, -3:], *first, "h")
+    ref.assert_within(z[:, -3:], *second, "z")
+    assert not h[:, :-3].any() and not z[:, :-3].any()
+
+
 def test_empty_and_refusals(cuda_device):
     from katz_b200 import KatzError, ops
     n = ops.Norm("rms")

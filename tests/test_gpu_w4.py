@@ -292,6 +292,28 @@ def test_linear_is_the_same_whatever_runs_around_it(cuda_device, M, N, K, zeros)
     assert ops.tc05_status() == 0
 
 
+def test_weights_past_four_gigabytes(cuda_device):
+    from katz_b200 import ops
+    g = _gen(12)
+    N, K, group = 270000, 32768, 128      # 4.4 GB of codes, 17.7 GB as fp16: byte and element offsets beyond 32 bits
+    q = torch.randint(0, 256, (N, K // 2), generator=g, device="cuda", dtype=torch.uint8)
+    scale = (0.004 * torch.exp(0.3 * torch.randn(N, K // group, generator=g, device="cuda"))).bfloat16()
+    wide = torch.randn(40, K + 8, generator=g, device="cuda").half()
+    ends = [slice(0, 200), slice(N - 333, N)]
+    for x in (wide[:2, :K], wide[:2, 1:K + 1], wide[:12, :K], wide[:40, :K]):      # streamed, direct, few rows, tcgen05
+        out = ops.linear_w4(x, q, scale, group=group)
+        for e in ends:
+            ref.assert_within(out[:, e], *ref.linear(x, q[e], scale[e], None, group, None, None, False, 1.0), "M=%d" % x.shape[0])
+    w = ops.dequantize_w4(q, scale, group=group)
+    for e in ends:
+        assert torch.equal(w[e], ref.weights(q[e], scale[e], None, group).half())
+    q2, scale2 = ops.quantize_w4(w, group=group)
+    for e in ends:
+        c, s = ref.quantize(w[e], group)
+        assert torch.equal(ref.codes(q2[e]), c) and torch.equal(scale2[e], s)
+    assert ops.tc05_status() == 0
+
+
 def test_adapter_switch_on_four_bit_weights(cuda_device):
     """The operators as an adapter switch uses them: merge in fp16, remake the 4-bit form in place, multiply; then back."""
     from collections import OrderedDict
