@@ -9,8 +9,8 @@
 // arithmetic is packed (two fp32 lanes an instruction). A row stays in registers from the load to the store; statistics are
 // fp32, of the values before any rounding (z is computed from the unrounded h), and the variance is the mean of squared
 // differences from the mean, so a row whose mean is large loses nothing. Rows of up to 1280 channels belong to one warp (sums
-// by shuffles, no barrier), longer ones to 4 or 16 warps. Measured: 32768 rows of 640 channels with an fp32 stream 45.6 us for
-// 252 MB (5.5 TB/s), 2048 x 1280 with gate, scale and shift 5.2 us (21 MB).
+// by shuffles, no barrier), longer ones to 4 or 16 warps. Measured: 32768 rows of 640 channels with an fp32 stream 44.5 us for
+// 252 MB (5.7 TB/s), 2048 x 1280 with gate, scale and shift 4.7 us (21 MB).
 #include "tc05.cuh"      // packed fp32 arithmetic
 
 namespace katz {

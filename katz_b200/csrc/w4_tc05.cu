@@ -19,8 +19,8 @@
 // CTA pairs (PAIR): the MMA covers 256 weight rows, 128 from each CTA's tensor memory, and each CTA loads half of x's tile:
 // per 64 k an SM then fetches BT * 64 + 4096 bytes instead of BT * 128 + 4096, where L2 was the bound.
 //
-// Measured (rows x N x K): 154 x 166400 x 2048 90 us = 1160 TFLOP/s (1180 before the clock falls; 1374 is cuBLAS's sustained rate),
-// the tensor pipe 69% busy; 2048 x 1280 x 5120 with a residual 24.7 us, 77 x 5120 x 1280 8.4 us, of which 5 us are what any
+// Measured (rows x N x K): 154 x 166400 x 2048 88 us = 1190 TFLOP/s (1374 is cuBLAS's sustained rate),
+// the tensor pipe 69% busy; 2048 x 1280 x 5120 with a residual 24.4 us, 77 x 5120 x 1280 8.4 us, of which 5 us are what any
 // launch of this kernel takes (set-up, first loads, the fill of the rings and the epilogue: 77 x 1280 x 256 takes 5.0 us).
 // Bound, where there are tiles for all SMs, by tensor pipe and unpacking together, which take about equally long.
 //
