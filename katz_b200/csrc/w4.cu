@@ -11,7 +11,7 @@ using namespace w4;
 
 // ---------------------------------------------------------------------------------------------------------------------
 // fp16 -> codes and scales. Per group: scale = bf16(max |w| / 7), code = 8 + rint(w / scale) with ties to even. The quotient
-// is the correctly rounded one (a product with the reciprocal and one residual step): w and scale have 11 and 8 significant
+// is the correctly rounded one (a product with the reciprocal and Markstein's residual correction): w and scale have 11 and 8 significant
 // bits, so a quotient that is not exactly half way between two codes is at least 2^-13 of its size away from there, and one
 // that is comes out exact. |w / scale| <= 7 * (1 + 2^-8): no code leaves 1..15.
 // A group that holds an infinity or a NaN gets a NaN scale: what is read back of it is NaN, never a plausible number.

@@ -27,6 +27,7 @@
 // Every mbarrier wait is bounded (tc05.cuh): on a time-out the CTA records a status word, stops storing, frees its TMEM and
 // returns; the host reads the word with katz_tc05_status().
 #include <algorithm>
+#include <mutex>
 #include <type_traits>
 
 #include "tc05.cuh"
@@ -482,7 +483,7 @@ __global__ void __launch_bounds__(WT_THREADS, 1) linear_w4_tc05_kernel(const __g
                     uint32_t r[16];
                     tmem_ld_32x16(tacc + 16 * i, r);
                     tmem_ld_wait();
-                    const uint32_t to = mapa_shared(sums + (slot * (t.split - 1) + part - (part > owner)) * 8192 + row * 4, owner);
+                    const uint32_t to = mapa_shared(sums + (slot * (t.split - 1) + part - ((int)owner < (int)part)) * 8192 + row * 4, owner);
 #pragma unroll
                     for (int e = 0; e < 16; ++e) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + e * 512), "r"(r[e]) : "memory");
                 }
@@ -664,6 +665,8 @@ struct W4Device {
 
 static int device_limits(W4Device& out) {
     static W4Device cached[KATZ_MAX_DEVICES] = {};
+    static std::mutex first_calls;      // callers' threads hold no lock of ours
+    std::lock_guard<std::mutex> lock(first_calls);
     W4Device& d = cached[current_device_index()];
     if (!d.ready) {
         W4Device found{};
@@ -722,7 +725,7 @@ int linear_w4_tc05(const W4Params& p, cudaStream_t st) {
             const long long tiles = (long long)m_tiles * n_tiles;
             if (two ? p.N <= 128 : bt > 192) continue;      // a lone CTA has room for two stages of wider x only
             const int slots = dev.slots[two ? 1 : mode];
-            if (split > 1 && (tiles > slots || units < 2 * split)) continue;
+            if (slots < 1 || (split > 1 && (tiles > slots || units < 2 * split))) continue;
             const int x_bytes = bt * (two ? 128 : 256);
             if ((WT_MAX_SMEM - WT_FIXED_SMEM - sums_bytes(bt, split)) / x_bytes < 2) continue;
             const int n_acc = bt <= 160 && tiles > slots ? 2 : 1;      // three stages of 64 columns beside two accumulators

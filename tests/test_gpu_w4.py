@@ -292,6 +292,31 @@ def test_linear_is_the_same_whatever_runs_around_it(cuda_device, M, N, K, zeros)
     assert ops.tc05_status() == 0
 
 
+def test_linear_from_threads(cuda_device):
+    import threading
+
+    from katz_b200 import ops
+    g = _gen(13)
+    q, scale, _ = _weight(g, 1280, 1280, 64, False)
+    xs = [torch.randn(m, 1280, generator=g, device="cuda").half() for m in (1, 8, 77, 600)]
+    want = [ops.linear_w4(x, q, scale) for x in xs]
+    torch.cuda.synchronize()
+    equal = []
+
+    def work():
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            outs = [ops.linear_w4(x, q, scale) for _ in range(30) for x in xs]
+        stream.synchronize()
+        equal.append(all(torch.equal(o, w) for o, w in zip(outs, want * 30)))
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert equal == [True] * 4 and ops.tc05_status() == 0
+
+
 def test_weights_past_four_gigabytes(cuda_device):
     from katz_b200 import ops
     g = _gen(12)
