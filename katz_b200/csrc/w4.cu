@@ -163,7 +163,7 @@ static PieceGrid piece_grid(int N, int K, int group, long long ldw) {
 // warp streams its codes through a ring in shared memory with asynchronous copies, across row tiles, every lane reading back
 // what it copied itself: HBM's latency needs some 45 KB in flight an SM. Scales and zero points of a tile lie in shared memory,
 // copied row by row while the tile before is multiplied. 1 x 5120 x 5120: 9.0 us (direct 11.2), 1 x 16384 x 8192 with groups of
-// 128: 20 us (direct 31; the codes alone at HBM's rate: 10), 1 x 32768 x 8192: 36 us (direct 59). Above HBM's rate it is bound
+// 128: 20 us (direct 31; the codes alone at HBM's rate: 10), 1 x 32768 x 8192: 32 us (direct 59). Above HBM's rate it is bound
 // by instructions: some 200 a block and warp (72 turn codes into operands, 8 multiply), the issue slots 64% busy, DRAM 34%.
 // Where the group is a block (128), the products take the integers code - zero and the scale multiplies their fp32 sum;
 // smaller groups differ from lane to lane, and the scale multiplies the operand (w4.cuh; on the whole block it costs 10% more).
@@ -199,15 +199,16 @@ __device__ __forceinline__ uint4 load_x_pairs(const __half* src, bool aligned) {
 // slots of 1 KB in shared memory. A lane copies, and reads back, its words of weight rows g and g + 8.
 struct CodeStream {
     const W4Params& p;
-    const int blocks, tiles, warps, warp, g, t;
+    const int blocks, tiles, warps, warp, hop, g, t;
     const uint32_t at;      // this lane's place in slot 0
     int tile, kb;           // the next block to copy
     uint32_t write_slot = 0, read_slot = 0;
     const unsigned char* src[2];      // this lane's codes of it
 
-    __device__ __forceinline__ CodeStream(const W4Params& p_, uint32_t ring)
-        : p(p_), blocks((p_.K + 127) / 128), tiles((p_.N + 15) / 16), warps(blockDim.x >> 5), warp(threadIdx.x >> 5),
-          g((threadIdx.x & 31) >> 2), t(threadIdx.x & 3), at(ring + warp * W4_RING * 1024 + (threadIdx.x & 31) * 16), tile(blockIdx.x), kb(warp) {
+    // warps_ of the CTA's share a tile, this is warp_ of them; hop_: from this warp's tile to its next
+    __device__ __forceinline__ CodeStream(const W4Params& p_, uint32_t ring, int warps_, int warp_, int tile_, int hop_)
+        : p(p_), blocks((p_.K + 127) / 128), tiles((p_.N + 15) / 16), warps(warps_), warp(warp_), hop(hop_), g((threadIdx.x & 31) >> 2),
+          t(threadIdx.x & 3), at(ring + (threadIdx.x >> 5) * W4_RING * 1024 + (threadIdx.x & 31) * 16), tile(tile_), kb(warp_) {
         at_tile();
     }
     __device__ __forceinline__ void at_tile() {
@@ -226,7 +227,7 @@ struct CodeStream {
             src[1] += warps * 64;
             if (kb >= blocks) {
                 kb = warp;
-                tile += gridDim.x;
+                tile += hop;
                 at_tile();
             }
         }
@@ -266,18 +267,18 @@ static ScaleRows scale_rows(const W4Params& p, int warps) {
     s.async_zero = p.J % 4 == 0 && ((uintptr_t)p.zero & 3) == 0;
     return s;
 }
-static long long scale_rows_bytes(const W4Params& p, int warps) {
+static long long scale_rows_bytes(const W4Params& p, int warps, int teams) {
     const ScaleRows s = scale_rows(p, warps);
-    return (s.ahead + 1ll) * 16 * (s.sld * 2 + (p.zero ? s.zld : 0));
+    return (s.ahead + 1ll) * 16 * teams * (s.sld * 2 + (p.zero ? s.zld : 0));
 }
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
-template <bool ZERO>
-__device__ __forceinline__ void read_scales(const W4Params& p, const ScaleRows& s, int tile, unsigned short* scales, unsigned char* zeros) {
+template <bool ZERO, int ROWS>
+__device__ __forceinline__ void read_scales(const W4Params& p, const ScaleRows& s, int n0, unsigned short* scales, unsigned char* zeros) {
     const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
-    for (int r = threadIdx.x >> 5; r < 16; r += warps) {
-        const size_t at = (size_t)min(tile * 16 + r, p.N - 1) * p.J;
+    for (int r = threadIdx.x >> 5; r < ROWS; r += warps) {
+        const size_t at = (size_t)min(n0 + r, p.N - 1) * p.J;
         if (s.async_scale) {
             for (int j = 2 * lane; j < p.J; j += 64) copy4(smem_u32(scales + r * s.sld + j), p.scale + at + j);
         } else {
@@ -372,22 +373,25 @@ __global__ void __launch_bounds__(W4_ROWS_THREADS) linear_w4_direct_kernel(const
     }
 }
 
-template <bool WIDE, bool ZERO>
+template <bool WIDE, bool ZERO, int TEAMS>
 __global__ void __launch_bounds__(W4_ROWS_THREADS) linear_w4_stream_kernel(const __grid_constant__ W4Params p, const ScaleRows sr, bool xaligned) {
     extern __shared__ __align__(16) unsigned char rows_smem[];
-    constexpr int LD = 16 + 4;
-    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    constexpr int LD = 16 + 4, ROWS = 16 * TEAMS;
+    const int all = blockDim.x >> 5, self = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int warps = all / TEAMS, team = TEAMS > 1 && self >= warps ? 1 : 0, warp = self - team * warps;      // of the tile's
+    const int hop = gridDim.x * TEAMS;
     const int sld = sr.sld, blocks = (p.K + 127) / 128, xld = x_row_bytes(p.K), tiles = (p.N + 15) / 16;
     unsigned char* xs = rows_smem;                                                        // [M][xld]
     unsigned char* ring = xs + p.M * xld;                                                 // [warp][W4_RING][2 rows][lane][16 bytes]
-    float* red = reinterpret_cast<float*>(ring + warps * W4_RING * 1024);                 // [warp][8][LD]
-    unsigned short* scales = reinterpret_cast<unsigned short*>(red + warps * 8 * LD);      // [ahead + 1][16][sld]
-    unsigned char* zeros = reinterpret_cast<unsigned char*>(scales + (sr.ahead + 1) * 16 * sld);      // [ahead + 1][16][zld]
-    CodeStream codes(p, smem_u32(ring));
+    float* red = reinterpret_cast<float*>(ring + all * W4_RING * 1024);                 // [warp][8][LD]
+    unsigned short* scales = reinterpret_cast<unsigned short*>(red + all * 8 * LD);      // [ahead + 1][rows][sld]
+    unsigned char* zeros = reinterpret_cast<unsigned char*>(scales + (sr.ahead + 1) * ROWS * sld);      // [ahead + 1][rows][zld]
+    CodeStream codes(p, smem_u32(ring), warps, warp, blockIdx.x * TEAMS + team, hop);
     pdl_wait();
     pdl_launch_dependents();
     for (int a = 0; a < sr.ahead; ++a)
-        if ((int)blockIdx.x + a * (int)gridDim.x < tiles) read_scales<ZERO>(p, sr, blockIdx.x + a * gridDim.x, scales + a * 16 * sld, zeros + a * 16 * sr.zld);
+        if ((int)blockIdx.x * TEAMS + a * hop < tiles)
+            read_scales<ZERO, ROWS>(p, sr, (blockIdx.x * TEAMS + a * hop) * 16, scales + a * ROWS * sld, zeros + a * ROWS * sr.zld);
     cp_async_commit();
     codes.start();
     for (int v = threadIdx.x; v < blocks * 16; v += blockDim.x) {
@@ -401,14 +405,14 @@ __global__ void __launch_bounds__(W4_ROWS_THREADS) linear_w4_stream_kernel(const
     // columns of x past the last row hold another row: what they give is not stored
     const uint32_t x_row = smem_u32(xs) + 16 * t + min(g, p.M - 1) * xld;
     int buf = 0;
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, buf = buf == sr.ahead ? 0 : buf + 1) {
-        const long long later = (long long)tile + (long long)sr.ahead * gridDim.x;
+    for (int tile = blockIdx.x * TEAMS; tile < tiles; tile += hop, buf = buf == sr.ahead ? 0 : buf + 1) {      // the first team's
+        const long long later = (long long)tile + (long long)sr.ahead * hop;
         const int into = buf == 0 ? sr.ahead : buf - 1;      // the buffer that the tile before has left
-        if (later < tiles) read_scales<ZERO>(p, sr, (int)later, scales + into * 16 * sld, zeros + into * 16 * sr.zld);
-        const unsigned short* s_row = scales + (buf * 16 + g) * sld;
-        const unsigned char* z_row = zeros + (buf * 16 + g) * sr.zld;
+        if (later < tiles) read_scales<ZERO, ROWS>(p, sr, (int)later * 16, scales + into * ROWS * sld, zeros + into * ROWS * sr.zld);
+        const unsigned short* s_row = scales + (buf * ROWS + team * 16 + g) * sld;
+        const unsigned char* z_row = zeros + (buf * ROWS + team * 16 + g) * sr.zld;
         float acc[2][4] = {};      // two chains of products
-        for (int kb = warp; kb < blocks; kb += warps) {
+        for (int kb = tile + team < tiles ? warp : blocks; kb < blocks; kb += warps) {
             uint32_t v[2][4];
             codes.next(v);
             const int j = min((kb * 128 + 32 * t) >> p.group_shift, p.J - 1);      // past the last k x is zero
@@ -454,13 +458,13 @@ __global__ void __launch_bounds__(W4_ROWS_THREADS) linear_w4_stream_kernel(const
         }
         cp_async_wait<W4_RING - 2>();      // the next tile's scales (and the next block)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) red[(warp * 8 + 2 * t + (e & 1)) * LD + g + 8 * (e >> 1)] = acc[0][e] + acc[1][e];
+        for (int e = 0; e < 4; ++e) red[(self * 8 + 2 * t + (e & 1)) * LD + g + 8 * (e >> 1)] = acc[0][e] + acc[1][e];
         __syncthreads();
-        for (int i = threadIdx.x; i < p.M * 16; i += blockDim.x) {
-            const int m = i / 16, nl = i % 16, n = tile * 16 + nl;
+        for (int i = threadIdx.x; i < p.M * ROWS; i += blockDim.x) {
+            const int m = i / ROWS, r = i - m * ROWS, of = r >> 4, nl = r & 15, n = tile * 16 + r;
             if (n >= p.N) continue;
             float v = 0.f;
-            for (int w = 0; w < warps; ++w) v += red[(w * 8 + m) * LD + nl];
+            for (int w = 0; w < warps; ++w) v += red[((of * warps + w) * 8 + m) * LD + nl];
             finish(p, WIDE ? v : v * OPERAND_UNSCALE, m, n);
         }
         __syncthreads();
@@ -489,23 +493,30 @@ static int launch_direct(const W4Params& p, bool xaligned, cudaStream_t st) {
     KATZ_LAUNCH_RET();
 }
 
-// shared memory of a CTA of the streaming kernel
-static long long stream_smem(const W4Params& p, int warps) {
-    return (long long)p.M * x_row_bytes(p.K) + (long long)warps * (W4_RING * 1024 + 8 * 20 * 4) + scale_rows_bytes(p, warps);
+// shared memory of a CTA of the streaming kernel: `teams` tiles at a time, `warps` on each
+static long long stream_smem(const W4Params& p, int warps, int teams) {
+    return (long long)p.M * x_row_bytes(p.K) + (long long)warps * teams * (W4_RING * 1024 + 8 * 20 * 4) + scale_rows_bytes(p, warps, teams);
 }
-// Warps of one, as many as share the blocks of k evenly; 0: x and the scales do not fit. Eight where four such CTAs fit an SM:
-// what a tile costs outside its blocks (barriers, sums) is spread over twice as many of them. With more x in shared memory
-// sixteen, if they fit.
-static int stream_warps(const W4Params& p) {
+struct StreamPlan {
+    int warps, teams;      // 0 warps: x and the scales do not fit
+};
+// Warps of a tile: as many as share its blocks of k evenly, up to eight or sixteen; what a tile costs outside its blocks
+// (barriers, sums) is spread over twice as many of them with eight. Eight where four such CTAs fit an SM. With more x in shared
+// memory two tiles of eight warps at a time, unless the SM with most work gets more tiles that way (1 x 32768 x 8192, groups of 128:
+// 14 tiles either way, 36.3 -> 32.3 us; 1 x 16384 x 8192: 8 tiles instead of 7, 20.1 -> 20.8), then sixteen.
+static StreamPlan stream_plan(const W4Params& p) {
     const int blocks = ceil_div(p.K, 128), eight = ceil_div(blocks, ceil_div(blocks, 8)), sixteen = ceil_div(blocks, ceil_div(blocks, 16));
-    if (stream_smem(p, eight) > 232448) return 0;
-    return 4 * (stream_smem(p, eight) + 1024) <= 233472 || stream_smem(p, sixteen) > 232448 ? eight : sixteen;
+    const int tiles = ceil_div(p.N, 16), sms = sm_count();
+    if (stream_smem(p, eight, 1) > 232448) return {0, 0};
+    if (4 * (stream_smem(p, eight, 1) + 1024) <= 233472) return {eight, 1};
+    if (stream_smem(p, eight, 2) <= 232448 && 2 * ceil_div(tiles, 2 * sms) == ceil_div(tiles, sms)) return {eight, 2};
+    return {stream_smem(p, sixteen, 1) <= 232448 ? sixteen : eight, 1};
 }
 
-template <bool WIDE>
+template <bool WIDE, int TEAMS>
 static int launch_stream(const W4Params& p, int warps, bool xaligned, cudaStream_t st) {
-    const size_t smem = (size_t)stream_smem(p, warps);
-    auto kernel = p.zero ? linear_w4_stream_kernel<WIDE, true> : linear_w4_stream_kernel<WIDE, false>;
+    const size_t smem = (size_t)stream_smem(p, warps, TEAMS);
+    auto kernel = p.zero ? linear_w4_stream_kernel<WIDE, true, TEAMS> : linear_w4_stream_kernel<WIDE, false, TEAMS>;
     static bool attr_dev[KATZ_MAX_DEVICES][2] = {};
     bool& attr = attr_dev[current_device_index()][p.zero != nullptr];
     if (!attr) {
@@ -514,8 +525,8 @@ static int launch_stream(const W4Params& p, int warps, bool xaligned, cudaStream
         attr = true;
     }
     // resident CTAs: 228 KB of shared memory an SM (1 KB of it per CTA), 64 registers a thread
-    const int per_sm = std::max(1, std::min(1024 / (warps * 32), (int)(233472 / (smem + 1024))));
-    launch_k(kernel, std::min(ceil_div(p.N, 16), sm_count() * per_sm), warps * 32, smem, st, p, scale_rows(p, warps), xaligned);
+    const int per_sm = std::max(1, std::min(1024 / (warps * TEAMS * 32), (int)(233472 / (smem + 1024))));
+    launch_k(kernel, std::min(ceil_div(p.N, 16 * TEAMS), sm_count() * per_sm), warps * TEAMS * 32, smem, st, p, scale_rows(p, warps), xaligned);
     KATZ_LAUNCH_RET();
 }
 
@@ -585,8 +596,11 @@ extern "C" int katz_linear_w4_f16(const katz_linear_w4_args* a, void* stream) {
     const bool tc05 = xaligned && K >= W4_TC05_MIN_K;
     const long long weights = (long long)N * K;
     const bool streams = M <= 8 && K > 1280 && weights > 3000000;
-    const int warps = streams ? stream_warps(p) : 0;      // 0: too much of x for shared memory
-    if (warps) return shift == 7 ? launch_stream<true>(p, warps, xaligned, st) : launch_stream<false>(p, warps, xaligned, st);
+    const StreamPlan plan = streams ? stream_plan(p) : StreamPlan{0, 0};
+    if (plan.warps) {
+        if (shift == 7) return plan.teams == 2 ? launch_stream<true, 2>(p, plan.warps, xaligned, st) : launch_stream<true, 1>(p, plan.warps, xaligned, st);
+        return plan.teams == 2 ? launch_stream<false, 2>(p, plan.warps, xaligned, st) : launch_stream<false, 1>(p, plan.warps, xaligned, st);
+    }
     if (tc05 && (M > 16 || streams || (M > 8 && weights > (K > 1280 ? 8000000 : 14000000)))) return linear_w4_tc05(p, st);
     return M <= 8 ? launch_direct<1>(p, xaligned, st) : launch_direct<2>(p, xaligned, st);
 }
