@@ -716,7 +716,7 @@ int linear_w4_tc05(const W4Params& p, cudaStream_t st) {
     W4Tile t{};
     bool pair = false;
     double best = 1e30;
-    const int min_tiles = ceil_div(p.M, 256);
+    const int min_tiles = ceil_div(p.M, p.N <= 128 ? 192 : 256);      // up to 128 weight rows are no pair's
     for (int mt = min_tiles; mt <= min_tiles + 8; ++mt) {
         const int bt = ceil_div(ceil_div(p.M, mt), 16) * 16, m_tiles = ceil_div(p.M, bt);
         for (int mode = -1; mode < 4; ++mode) {      // -1: pairs; i: K split over 2^i CTAs

@@ -128,6 +128,19 @@ def test_linear_edges(cuda_device, M, N, K):
     _linear_case(M, N, K, group=(32, 64, 128)[(M + N + K // 32) % 3], zeros=(M + N) % 2 == 0, bias=N % 2 == 0, seed=N + K)
 
 
+# the same kinds of sizes where the tcgen05 kernel takes them: more work, odd numbers of rows on either side, short last steps
+@pytest.mark.parametrize("M", [17, 31, 64, 77, 129, 257, 600])
+@pytest.mark.parametrize("N,K,group,zeros", [(5123, 1312, 32, True), (2051, 2400, 64, False), (10003, 416, 128, False), (1283, 7200, 32, False)])
+def test_linear_more_rows(cuda_device, M, N, K, group, zeros):
+    _linear_case(M, N, K, group=group, zeros=zeros, bias=M % 2 == 0, residual=M > 60, silu=M == 77, out_scale=0.5 if M == 129 else 1.0, seed=M)
+
+
+@pytest.mark.parametrize("N", [15, 16, 127, 128, 129, 257])
+@pytest.mark.parametrize("K", [1440, 4128])
+def test_linear_many_rows_of_few_weights(cuda_device, N, K):
+    _linear_case(8000, N, K, group=64, bias=True, residual=True, seed=N)
+
+
 @pytest.mark.parametrize("M,N,K", [(2, 13760, 1280), (1, 16384, 8192), (8, 10240, 1280), (77, 5120, 1280), (154, 20480, 2048),
                                    (2048, 1280, 5120), (300, 5120, 10240)])
 def test_linear_sizes_of_the_step(cuda_device, M, N, K):
