@@ -590,9 +590,11 @@ extern "C" int katz_linear_w4_f16(const katz_linear_w4_args* a, void* stream) {
     cudaStream_t st = (cudaStream_t)stream;
     // Up to eight rows: direct while a warp's whole reduction is in flight at once or the weights are few, else streamed (weights
     // cold, direct / streamed, one row: 1280 x 1280 2.3 / 3.1 us, 40960 x 1280 13.9 / 14.1, 640 x 4096 3.6 / 3.8, 2560 x 2560
-    // 6.2 / 5.0, 1280 x 5120 7.0 / 5.2, 8192 x 10240 21 / 17). Up to sixteen rows: direct while the weights are few, else the
-    // tcgen05 kernel (direct / tcgen05, 16 rows: 1280 x 1280 3.1 / 6.7, 10240 x 1280 7.7 / 8.8, 13760 x 1280 13.4 / 9.2, 1280 x
-    // 5120 9.2 / 9.0, 2560 x 5120 13.5 / 9.9). x that TMA cannot read takes the direct kernel at any size.
+    // 6.2 / 5.0, 1280 x 5120 7.0 / 5.2, 8192 x 10240 21 / 17). More rows: direct while the rows, in sixteens, times the weights
+    // are so few that the tcgen05 kernel's fixed 5 us are the longer (direct / tcgen05, rows x N x K: 77 x 640 x 640 3.2 / 7.4 us,
+    // 300 x 320 x 320 3.2 / 6.7, 512 x 1280 x 320 8.3 / 7.0, 16 x 1280 x 1280 3.1 / 6.7, 64 x 1280 x 1280 5.2 / 7.0, 128 x 1280 x
+    // 1280 7.1 / 7.6, 77 x 2560 x 1280 10.8 / 8.3, 16 x 10240 x 1280 7.7 / 8.8, 48 x 640 x 2560 4.6 / 7.0, 32 x 1280 x 2560 8.1 /
+    // 7.3, 16 x 2560 x 5120 13.5 / 9.9). x that TMA cannot read takes the direct kernel at any size.
     const bool tc05 = xaligned && K >= W4_TC05_MIN_K;
     const long long weights = (long long)N * K;
     const bool streams = M <= 8 && K > 1280 && weights > 3000000;
@@ -601,6 +603,7 @@ extern "C" int katz_linear_w4_f16(const katz_linear_w4_args* a, void* stream) {
         if (shift == 7) return plan.teams == 2 ? launch_stream<true, 2>(p, plan.warps, xaligned, st) : launch_stream<true, 1>(p, plan.warps, xaligned, st);
         return plan.teams == 2 ? launch_stream<false, 2>(p, plan.warps, xaligned, st) : launch_stream<false, 1>(p, plan.warps, xaligned, st);
     }
-    if (tc05 && (M > 16 || streams || (M > 8 && weights > (K > 1280 ? 8000000 : 14000000)))) return linear_w4_tc05(p, st);
+    const long long work = (long long)ceil_div(M, 16) * weights;
+    if (tc05 && (M > 8 ? work > (K > 1280 ? 6000000 : K > 640 ? 14000000 : 10000000) : streams)) return linear_w4_tc05(p, st);
     return M <= 8 ? launch_direct<1>(p, xaligned, st) : launch_direct<2>(p, xaligned, st);
 }
